@@ -22,12 +22,13 @@ RuntimeError) with the same messages.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
-from ._capi import DeviceStatus, HsbError, KeyView, LayerBuffers, Selection, lib
+from ._capi import DeviceStatus, HsbError, KeyView, KvPages, LayerBuffers, Selection, lib
 
 __all__ = [
     "HsbError", "InvalidArgument", "FullGqaScorer", "score_full_gqa", "score_pipeline_v3",
@@ -36,11 +37,14 @@ __all__ = [
     "attention_dense", "rehearsal_query", "GQAPrefetchCuda", "GQADeliveryWorkspace",
     "SelectedKVLayer", "attention_slots", "h2o_group_sums", "GQAH2OStatsCuda",
     "segment_header", "segment_extent_bytes", "kv_records_encode", "kv_records_verify", "kv_read_plan",
-    "kv_read_groups", "plan_hot_slots", "score_history", "History", "DecodeExecutor",
+    "kv_read_groups", "plan_hot_slots", "score_history", "History", "DecodeExecutor", "KVPages",
 ]
 
 # Status codes the reference reports as std::invalid_argument.
-_INVALID_ARGUMENT = {10, 11, 12, 30, 31, 40, 41, 42, 43, 93}
+_INVALID_ARGUMENT = {10, 11, 12, 30, 31, 40, 41, 42, 43, 93, 120, 121, 122}
+
+
+_HERE = contextlib.nullcontext()
 
 
 class InvalidArgument(HsbError, ValueError):
@@ -704,6 +708,169 @@ class DecodeExecutor:
                                                C.c_float(self.ratio), self.count, C.byref(b), _ptr(out),
                                                _ptr(self.status), _stream(stream)))
         self.completed[layer] += 1
+        return out
+
+
+# ------------------------------------------------------- paged KV cache
+class KVPages:
+    """A pool of 64-token K/V pages (hsb_kv_*): F16, or int8 / e4m3 codes with
+    a scale per row that are made as rows are written.  ``data`` is the pool,
+    uint8 [pages, kv_heads, page bytes]; page tables are int32 [batch, width]
+    (entries behind a sequence's last page may be anything), lengths and
+    starts int32 [batch].  Calls enqueue on ``stream`` (the device's current
+    one) and never synchronise; what only the GPU can see -- a table entry
+    outside the pool, a position behind the table, a non-finite value written
+    -- is kept in ``status`` until ``check`` raises it."""
+
+    FORMATS = {"f16": 0, "int8": 1, "e4m3": 2}
+    PAGE_TOKENS = 64
+
+    def __init__(self, pages: int = 0, kv_heads: int = 8, format: str = "int8", device="cuda", data=None):
+        torch = _torch()
+        if format not in self.FORMATS:
+            raise InvalidArgument(120, "unknown paged KV format")
+        if kv_heads not in (1, 2, 4, 8):
+            raise InvalidArgument(120, "paged KV heads must be 1, 2, 4 or 8")
+        self.format, self.kv_heads = format, int(kv_heads)
+        size = lib().hsb_kv_page_bytes(self.FORMATS[format])
+        if data is None:
+            if pages < 1:
+                raise InvalidArgument(120, "a paged KV pool has at least one page")
+            data = torch.empty((int(pages), self.kv_heads, size), dtype=torch.uint8, device=device)
+        if data.dtype != torch.uint8 or data.dim() != 3 or tuple(data.shape[1:]) != (self.kv_heads, size) or \
+                data.shape[0] < 1 or not data.is_contiguous():
+            raise InvalidArgument(120, f"a {format} pool is uint8 [pages, {self.kv_heads}, {size}], contiguous")
+        if data.device.type != "cuda":
+            raise InvalidArgument(120, "a paged KV pool is CUDA device memory")
+        self.data, self.pages, self.device = data, int(data.shape[0]), data.device
+        self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        self._c = KvPages(data.data_ptr(), self.pages, self.FORMATS[format], self.kv_heads)
+        self._ref, self._st = C.byref(self._c), C.c_void_p(self.status.data_ptr())
+
+    def check(self, stream=None) -> None:
+        """Synchronises; raises (and forgets) what the calls so far recorded."""
+        try:
+            with _torch().cuda.device(self.device):
+                _check_status(self.status, stream if stream is not None else _torch().cuda.current_stream(self.device))
+        except HsbError:
+            self.status.zero_()
+            raise
+
+    def _arg(self, t, name: str, dtypes: tuple, shape: tuple) -> int:
+        """Address of a contiguous tensor on the pool's device; -1 in shape: any extent."""
+        if t.device != self.device:
+            raise InvalidArgument(120, f"{name} must be on the pool's device, {self.device}")
+        if t.dtype not in dtypes:
+            raise InvalidArgument(120, f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, not {str(t.dtype)[6:]}")
+        if t.dim() != len(shape) or any(w not in (-1, n) for w, n in zip(shape, t.shape)) or not t.is_contiguous():
+            raise InvalidArgument(120, f"{name} must be {list(shape)}, contiguous; got {list(t.shape)}")
+        return t.data_ptr()
+
+    def _table(self, table, batch: int = -1) -> tuple:
+        torch = _torch()
+        at = self._arg(table, "table", (torch.int32,), (batch, -1))
+        if table.numel() == 0:
+            raise InvalidArgument(120, "an empty page table")
+        return at, table.shape[1], table.shape[0]
+
+    def _on(self, stream):
+        """A context in which new tensors belong to the stream of the call, and the stream."""
+        torch = _torch()
+        if stream is None:
+            if torch.cuda.current_device() == self.device.index:
+                return _HERE, torch.cuda.current_stream(self.device).cuda_stream
+            return torch.cuda.device(self.device), torch.cuda.current_stream(self.device).cuda_stream
+        if stream.device != self.device:
+            raise InvalidArgument(120, f"the stream must be on the pool's device, {self.device}")
+        return torch.cuda.stream(stream), stream.cuda_stream
+
+    def append(self, rows, table, starts, offsets=None, stream=None) -> None:
+        """Writes 16-bit float rows [n, 2 (K, V), kv_heads, 128] (any strides that
+        are multiples of 8 over the first three axes).  Sequence b's are
+        [offsets[b], offsets[b + 1]) (int32 [batch + 1]) at positions starts[b]
+        onwards; without offsets row i is sequence i's next token."""
+        torch = _torch()
+        tp, width, batch = self._table(table)
+        sp = self._arg(starts, "starts", (torch.int32,), (batch,))
+        op = 0 if offsets is None else self._arg(offsets, "offsets", (torch.int32,), (batch + 1,))
+        if rows.device != self.device or rows.dtype not in (torch.float16, torch.int16) or \
+                rows.dim() != 4 or tuple(rows.shape[1:]) != (2, self.kv_heads, 128) or rows.stride(3) != 1:
+            raise InvalidArgument(120, f"rows must be float16 [n, 2, {self.kv_heads}, 128] on {self.device}")
+        n = rows.shape[0]
+        if n == 0:
+            if offsets is None:
+                raise InvalidArgument(120, "without offsets there is one row per sequence")
+            return
+        # (an axis of one element may have any stride)
+        k, s0 = rows.data_ptr(), rows.stride(0) if n > 1 else 0
+        s2 = rows.stride(2) if self.kv_heads > 1 else 0
+        context, s = self._on(stream)
+        with context:
+            _raise(lib().hsb_kv_append(self._ref, tp, width, batch, sp, op, k, k + 2 * rows.stride(1), n, s0, s2,
+                                       self._st, s))
+
+    def read(self, positions, table, seqs=None, count=None, out=None, stream=None):
+        """F16 rows [n, 2, kv_heads, 128] of positions (int32 [n]) of sequences
+        seqs (int32 [n]; sequence 0 without them).  count (int32 [1], on the
+        device): only the first count rows are written."""
+        torch = _torch()
+        tp, width, batch = self._table(table)
+        pp = self._arg(positions, "positions", (torch.int32, torch.uint32), (-1,))
+        n = positions.shape[0]
+        qp = 0 if seqs is None else self._arg(seqs, "seqs", (torch.int32,), (n,))
+        cp = 0 if count is None else self._arg(count, "count", (torch.int32, torch.uint32), (1,))
+        context, s = self._on(stream)
+        with context:
+            if out is None:
+                out = torch.empty((n, 2, self.kv_heads, 128), dtype=torch.float16, device=self.device)
+            dst = self._arg(out, "out", (torch.float16, torch.int16), (n, 2, self.kv_heads, 128))
+            if n:
+                _raise(lib().hsb_kv_read(self._ref, tp, width, batch, qp, pp, cp, n, dst, self._st, s))
+        return out
+
+    def attention(self, q, table, lengths, out=None, stream=None):
+        """softmax(q . K / sqrt(128)) V over each sequence's first lengths[b]
+        positions: q, out F32 [batch, 4 * kv_heads, 128]; zero for an empty one."""
+        torch = _torch()
+        tp, width, batch = self._table(table)
+        shape = (batch, 4 * self.kv_heads, 128)
+        qp = self._arg(q, "q", (torch.float32,), shape)
+        np_ = self._arg(lengths, "lengths", (torch.int32,), (batch,))
+        context, s = self._on(stream)
+        with context:
+            if out is None:
+                out = torch.empty(shape, dtype=torch.float32, device=self.device)
+            dst = self._arg(out, "out", (torch.float32,), shape)
+            size = lib().hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            _raise(lib().hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size, self._st, s))
+        return out
+
+    def attention_shared(self, q, table, lengths, prefix: "KVPages", prefix_table, prefix_tokens: int, out=None,
+                         stream=None):
+        """attention for a batch whose sequences share their first
+        prefix_tokens positions, kept in an F16 pool and read once for all;
+        table and lengths are of each sequence's own tokens.  q, out F16."""
+        torch = _torch()
+        tp, width, batch = self._table(table)
+        shape = (batch, 4 * self.kv_heads, 128)
+        qp = self._arg(q, "q", (torch.float16,), shape)
+        np_ = self._arg(lengths, "lengths", (torch.int32,), (batch,))
+        ptp = prefix._arg(prefix_table, "prefix_table", (torch.int32,), (-1,))
+        prefix_tokens = int(prefix_tokens)
+        if prefix.device != self.device:
+            raise InvalidArgument(120, "the prefix must be on the pool's device")
+        if prefix_tokens < 1 or prefix_tokens > 64 * prefix_table.shape[0]:
+            raise InvalidArgument(120, "prefix_tokens must be 1 .. 64 * len(prefix_table)")
+        context, s = self._on(stream)
+        with context:
+            if out is None:
+                out = torch.empty(shape, dtype=torch.float16, device=self.device)
+            dst = self._arg(out, "out", (torch.float16,), shape)
+            size = lib().hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            _raise(lib().hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_, batch, qp,
+                                                 dst, ws.data_ptr(), size, self._st, s))
         return out
 
 

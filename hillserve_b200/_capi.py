@@ -47,6 +47,10 @@ class LayerBuffers(C.Structure):
     ]
 
 
+class KvPages(C.Structure):
+    _fields_ = [("data", P), ("pages", SZ), ("format", C.c_int), ("kv_heads", C.c_int)]
+
+
 # name: (restype, argtypes)
 _SIGNATURES = {
     "hsb_abi_version": (I, []),
@@ -120,6 +124,13 @@ _SIGNATURES = {
     "hsb_executor_query": (I, [P, P, P, P]),
     "hsb_executor_workspace_bytes": (SZ, [SZ, SZ]),
     "hsb_executor_decode_layer": (I, [P, P, P, P, SZ, SZ, I, F, F, SZ, P, P, P, P]),
+    "hsb_kv_page_bytes": (SZ, [I]),
+    "hsb_kv_append": (I, [P, P, SZ, SZ, P, P, P, P, SZ, SZ, SZ, P, P]),
+    "hsb_kv_read": (I, [P, P, SZ, SZ, P, P, P, SZ, P, P, P]),
+    "hsb_kv_attention_workspace_bytes": (SZ, [SZ, I]),
+    "hsb_kv_attention": (I, [P, P, SZ, P, SZ, P, P, P, SZ, P, P]),
+    "hsb_kv_attention_shared_workspace_bytes": (SZ, [SZ, I, SZ]),
+    "hsb_kv_attention_shared": (I, [P, P, SZ, P, P, SZ, P, SZ, P, P, P, SZ, P, P]),
     "hsb_synth_normal_f16": (I, [P, SZ, U64, F, P]),
     "hsb_synth_normal_bf16": (I, [P, SZ, U64, F, P]),
     "hsb_synth_keys": (I, [P, SZ, SZ, U64, F, F, I, F, P]),

@@ -129,6 +129,9 @@ const char* hsb_status_message(int status) {
     case HSB_E_EXECUTOR_NONFINITE_KV: return "GQA current model KV contains nonfinite F16";
     case HSB_E_EXECUTOR_REHEARSAL: return "full GQA rehearsal nonfinite";
     case HSB_E_EXECUTOR_REHEARSAL_F16: return "full GQA rehearsal F16 overflow";
+    case HSB_E_KV_SHAPE: return "paged KV shape, stride or alignment";
+    case HSB_E_KV_PAGE: return "paged KV table names a page outside the pool";
+    case HSB_E_KV_POSITION: return "paged KV position or length behind the table's end";
     default: return "unknown hsb status";
     }
 }

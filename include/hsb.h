@@ -109,7 +109,11 @@ typedef enum hsb_status {
     HSB_E_EXECUTOR_SHAPE = 110,
     HSB_E_EXECUTOR_NONFINITE_KV = 111,
     HSB_E_EXECUTOR_REHEARSAL = 112,
-    HSB_E_EXECUTOR_REHEARSAL_F16 = 113
+    HSB_E_EXECUTOR_REHEARSAL_F16 = 113,
+    /* paged KV cache (no counterpart in the reference) */
+    HSB_E_KV_SHAPE = 120,
+    HSB_E_KV_PAGE = 121,
+    HSB_E_KV_POSITION = 122
 } hsb_status;
 
 int hsb_abi_version(void);
@@ -620,6 +624,85 @@ int hsb_executor_decode_layer(const uint16_t* d_current, const float* d_rehearsa
                               uint16_t* d_cache, size_t capacity, size_t position, int dense, float alpha,
                               float ratio, size_t count, const hsb_layer_buffers* buffers, float* d_out,
                               hsb_device_status* d_status, void* stream);
+
+/* -------------------------------------------------------- paged KV cache
+ * The K/V cache of a served batch, in pages of 64 tokens, F16 or quantised to
+ * 8 bits as it is written (the reference keeps one sequence's F16 rows; these
+ * calls have no counterpart in it).  A pool is device memory
+ * [pages][kv_heads][hsb_kv_page_bytes(format)], 16-byte aligned, of any
+ * content: rows that were never written are never used.  kv_heads is 1, 2, 4
+ * or 8 (a KV-head shard holds its own), with four query heads each.
+ *
+ * A page of one KV head: K panels, V panels, then in the 8-bit formats the F32
+ * scales K[64], V[64].  A panel is 64 rows of 128 bytes; 16-byte chunk c of
+ * row r lies at place c ^ (r & 7).  F16 has two panels for K and two for V
+ * (channels 0-63, 64-127), int8 and e4m3 one each.  Of each row's 128 channels
+ * the 8-bit formats keep scale = max|x| / top and code = round(x * (top /
+ * max|x|)), top 127 (int8) or 448 (e4m3), in F32 with one rounding per
+ * operation, codes to nearest even; a code stands for code * scale.
+ *
+ * Position t of sequence b lives in row t % 64 of page d_table[b * table_width
+ * + t / 64].  Entries behind a sequence's last page are not read.  An entry
+ * outside the pool sets HSB_E_KV_PAGE, a position or length behind the table's
+ * end HSB_E_KV_POSITION, in *d_status (index = the row or sequence; d_status
+ * may be NULL): nothing outside the pool or the table is touched, the row is
+ * skipped (written) or zero (read), the page's tokens are left out of the
+ * attention, and a sequence of such a length counts as empty. */
+#define HSB_KV_F16 0
+#define HSB_KV_INT8 1
+#define HSB_KV_E4M3 2
+#define HSB_KV_PAGE_TOKENS 64
+typedef struct hsb_kv_pages {
+    void* data;
+    size_t pages;
+    int format;
+    int kv_heads;
+} hsb_kv_pages;
+/* Bytes of one page of one KV head; 0 for an unknown format. */
+size_t hsb_kv_page_bytes(int format);
+/* Writes (and quantises) F16 rows: row i of d_k / d_v starts at i *
+ * row_stride words, its KV head h at + h * head_stride (both multiples of 8,
+ * pointers 16-byte aligned): K||V rows are d_v = d_k + 128 * kv_heads,
+ * row_stride 256 * kv_heads, head_stride 128; the model's current tensor
+ * (hsb_executor_append) d_v = d_k + 128, head_stride 256.  Sequence b's rows
+ * are [d_offsets[b], d_offsets[b + 1]) (ascending, [batch + 1]) at positions
+ * d_starts[b] onwards; d_offsets NULL: row i is sequence i's next token
+ * (rows == batch).  Rows of no sequence are ignored.  A page belongs to one
+ * sequence while it is written: two rows of one call must not meet in one
+ * place.  A non-finite value sets HSB_E_EXECUTOR_NONFINITE_KV (index = row)
+ * and is kept as it is in F16; in 8 bits it takes no part in the scale, an
+ * infinity becomes the largest code and NaN 0. */
+int hsb_kv_append(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width, size_t batch,
+                  const int32_t* d_starts, const int32_t* d_offsets, const uint16_t* d_k, const uint16_t* d_v,
+                  size_t rows, size_t row_stride, size_t head_stride, hsb_device_status* d_status, void* stream);
+/* Reads rows back as F16 K||V rows (code * scale rounded to F32, then to
+ * F16), d_out [max_rows][2][kv_heads][128]: row i
+ * is position d_positions[i] of sequence d_seqs[i] (d_seqs NULL: sequence 0),
+ * i < *d_count (d_count NULL: max_rows); rows behind are left as they were.
+ * The paged counterpart of hsb_stage_rows: with hsb_union's outputs as
+ * d_positions and d_count it gives the payload rows of hsb_pack. */
+int hsb_kv_read(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width, size_t batch,
+                const int32_t* d_seqs, const uint32_t* d_positions, const uint32_t* d_count, size_t max_rows,
+                uint16_t* d_out, hsb_device_status* d_status, void* stream);
+/* Decode attention of a batch, one token per sequence: d_q, d_out F32
+ * [batch][4 kv_heads][128], out = softmax(q . K / sqrt(128)) V over positions
+ * [0, d_lengths[b]); zero for an empty sequence.  Grids depend on batch and
+ * table_width only, so a captured call follows lengths and tables as they
+ * change.  Workspace: as for the other stages, of one call at a time. */
+size_t hsb_kv_attention_workspace_bytes(size_t batch, int kv_heads);
+int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width, const int32_t* d_lengths,
+                     size_t batch, const float* d_q, float* d_out, void* d_workspace, size_t workspace_bytes,
+                     hsb_device_status* d_status, void* stream);
+/* The same for a batch whose sequences share their first prefix_tokens
+ * positions: prefix (an F16 pool) through d_prefix_table
+ * [ceil(prefix_tokens / 64)], read once for all of them, then each sequence's
+ * own d_lengths[b] tokens in `pages` (any format; same kv_heads).  d_q, d_out
+ * F16.  prefix_tokens >= 1; an own length may be 0. */
+size_t hsb_kv_attention_shared_workspace_bytes(size_t batch, int kv_heads, size_t prefix_tokens);
+int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_table, size_t prefix_tokens,
+                            const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width,
+                            const int32_t* d_lengths, size_t batch, const uint16_t* d_q, uint16_t* d_out,
+                            void* d_workspace, size_t workspace_bytes, hsb_device_status* d_status, void* stream);
 
 /* ------------------------------------------------------ synthetic inputs
  * Benchmark inputs, not part of the reference interface, defined so that a
