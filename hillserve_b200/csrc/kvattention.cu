@@ -7,7 +7,7 @@
 // bits): the kernel is bound by the bytes of the pages, and is built to keep
 // them coming.  Page blocks arrive whole by bulk copies into a ring of shared
 // memory; warps take 32 tokens each, turn codes into F16 fragments in
-// registers (both formats convert exactly) and run both products with
+// registers (both formats convert exactly) and runs both products with
 // mma.sync.m16n8k16, tokens and channels in the wide dimension:
 //
 //   logits  S^T[token][col] = K[token][ch] . Q^T[ch][col]
@@ -19,12 +19,17 @@
 // long as both operands agree: each lane owns whole 16-byte chunks, so the
 // fragments are the loaded words themselves, with no ldmatrix.  The K scale
 // multiplies a token's logits, the V scale its weight, both in F32; weights
-// are brought to [0, 2^14] by a power of two before their split into halves.
+// are brought into F16's range by a power of two before their split into halves.
+// The running maximum is only moved when a logit passes it by 8 (in log2): until
+// then no reduction across the warp and no rescaling is needed.
 //
-// Work is split evenly without regard to lengths: the (sequence, head, page)
-// units in that order are one line, of which every CTA takes an equal stretch.
-// A (sequence, head) run inside one CTA is finished there; one that crosses
-// CTAs leaves F32 partials that kv_combine_kernel folds in order.
+// Work is split evenly without regard to lengths: the (sequence, head, page) units in that order are one line, of which every CTA takes an equal
+// stretch and each of its warps an equal part, with a ring of its own that it
+// fills itself.  Warps never wait for one another inside the line, so what a run
+// costs at its ends (its query, its last sums) hides behind the others' work.  A
+// (sequence, head) run inside one warp's part is finished there, one that crosses
+// warps is folded in shared memory at the end, and one that crosses CTAs leaves
+// F32 partials that kv_combine_kernel folds in order.
 #include <algorithm>
 #include <cmath>
 
@@ -33,22 +38,34 @@
 namespace hsb {
 namespace {
 
-constexpr int kOutPitch = kDim + 4;
-constexpr float kWeightTop = 16384.0f;  // 2^14: weights' F16 halves are at most this
+// Weights enter the second product as p x 2^7 (x the V scale over its
+// reference): p is at most 2^kSlack, so their F16 halves reach 2^15 at most.
+constexpr float kWeightUnit = 128.0f;
+constexpr float kSlack = 8.0f;
 
-// Warps 2 i and 2 i + 1 take the two halves of units i, i + kConsumers / 2, ...
-// The ring's length is a multiple of that step, so a stage has the same two
-// readers in every round: one that skipped a round could take the parity of a
-// later fill for that of an earlier one.
+#ifndef W8
+#define W8 8
+#define S8 3
+#define W16 8
+#define S16 3
+#endif
+// Each warp's ring holds K and V of its units in turn (K 0, V 0, K 1, ...): a
+// slot is free again as soon as its product is done.  A unit is a page in 8
+// bits; in F16, twice the bytes a token and no codes to convert, half a page.
 template <int F>
 struct Ring {
-    static constexpr int kConsumers = F == HSB_KV_F16 ? 6 : 8;
-    static constexpr int kThreads = (kConsumers + 1) * 32;
-    static constexpr int kStages = F == HSB_KV_F16 ? 6 : 12;
-    static_assert(kStages % (kConsumers / 2) == 0, "a stage keeps its readers");
-    static constexpr int kData = kStages * PageFormat<F>::kBytes;
-    static constexpr int kMerge = kConsumers * kGroup * (kOutPitch + 2) * 4;
-    static constexpr int kSmem = 128 + kData + kMerge;
+    using Fmt = PageFormat<F>;
+    static constexpr int kWarps = F == HSB_KV_F16 ? W16 : W8;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kSlots = F == HSB_KV_F16 ? S16 : S8;
+    static constexpr int kTokens = F == HSB_KV_F16 ? kPageTokens / 2 : kPageTokens;  // of a unit
+    static constexpr int kPerPage = kPageTokens / kTokens;
+    static constexpr int kPanel = kTokens * 128;
+    static constexpr int kScales = Fmt::kPanels * kPanel;
+    static constexpr int kSlot = kScales + (Fmt::kScaled ? kTokens * 4 : 0);
+    static constexpr int kSmem = 128 + kWarps * (kSlots * kSlot + kPartFloats * 4);
+    static_assert(kSlots * kSlot >= kPartFloats * 4, "a piece fits in a warp's ring");
+    __host__ __device__ static constexpr uint32_t units(uint32_t tokens) { return (tokens + kTokens - 1) / kTokens; }
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -76,18 +93,30 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ __half split_half(float x, bool low) {
-    const __half hi = __float2half_rn(x);
-    return low ? __float2half_rn(x - __half2float(hi)) : hi;
+// (a, b) as the F16 pair of this lane's columns: their roundings, or what these leave.
+__device__ __forceinline__ uint32_t split_pair(float a, float b, bool low) {
+    const __half2 hi = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(hi);
+    const __half2 lo = __floats2half2_rn(a - f.x, b - f.y);
+    return low ? *reinterpret_cast<const uint32_t*>(&lo) : *reinterpret_cast<const uint32_t*>(&hi);
 }
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-    return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16);
+__device__ __forceinline__ float4 load_q4(const float* q) { return *reinterpret_cast<const float4*>(q); }
+__device__ __forceinline__ float4 load_q4(const uint16_t* q) {
+    const uint2 w = *reinterpret_cast<const uint2*>(q);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
 }
-__device__ __forceinline__ float load_q(const float* q, size_t i) { return q[i]; }
-__device__ __forceinline__ float load_q(const uint16_t* q, size_t i) { return half_value(q[i]); }
+
+// 2^x; a result below the normal range is 0.
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Tokens of a sequence; a length behind the table's end counts as none.
-__device__ __forceinline__ unsigned long long tokens_of(const PagedAttention& p, unsigned long long b, bool report) {
+__device__ __forceinline__ uint32_t tokens_of(const PagedAttention& p, uint32_t b, bool report) {
     if (!p.lengths) return p.length;
     const int32_t n = p.lengths[b];
     if (n < 0 || (unsigned long long)n > p.v.width * kPageTokens) {
@@ -96,397 +125,424 @@ __device__ __forceinline__ unsigned long long tokens_of(const PagedAttention& p,
     }
     return n;
 }
-
-// A CTA's stretch of the line of units, one (sequence, head) run at a time.
+// A position in the line of units, up to `end`.
+template <typename R>
 struct Walker {
-    unsigned long long u, end;      // the stretch [u, end)
-    unsigned long long seq, tokens, pages;
-    unsigned long long run;         // first unit of the current run
+    uint32_t u, end;
+    uint32_t seq, tokens, units;  // of the current run
+    uint32_t run;                 // its first unit
     int head;
-    __device__ unsigned long long stop() const { return min(end, run + pages); }
-    __device__ void next(const PagedAttention& p) {
-        u = stop();
-        run += pages;
-        if (++head < p.v.heads || u >= end) return;
-        head = 0;
-        do {
-            ++seq;
-            tokens = tokens_of(p, seq, false);
-            pages = (tokens + kPageTokens - 1) / kPageTokens;
-        } while (pages == 0);
+    __device__ bool done() const { return u >= end; }
+    __device__ uint32_t run_end() const { return run + units; }
+    // Steps over one unit; true when that enters another run.
+    __device__ bool step(const PagedAttention& p) {
+        if (++u < run_end()) return false;
+        run += units;
+        if (++head == p.v.heads && !done()) {
+            head = 0;
+            do {
+                ++seq;
+                tokens = tokens_of(p, seq, false);
+                units = R::units(tokens);
+            } while (units == 0);
+        }
+        return true;
     }
 };
 
-// Finds CTA `cta`'s stretch of `ctas`.  Every thread of the block calls it.
-template <int kThreads>
-__device__ Walker find_stretch(const PagedAttention& p, unsigned cta, unsigned ctas, unsigned long long* total_units) {
-    __shared__ unsigned long long warp_sum_s[kThreads / 32];
-    __shared__ unsigned long long found[4];
+// Finds this warp's part of CTA blockIdx.x's stretch.  Every thread of the block calls it.
+template <typename R>
+__device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, uint32_t* stretch) {
+    constexpr int kThreads = R::kThreads, kWarps = R::kWarps;
+    __shared__ uint32_t warp_sum_s[kWarps], found[kWarps][3];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned long long per = (p.batch + kThreads - 1) / kThreads;
-    const unsigned long long b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-    unsigned long long mine = 0;
-    for (unsigned long long b = b0; b < b1; ++b)
-        mine += (tokens_of(p, b, cta == 0) + kPageTokens - 1) / kPageTokens;
-    unsigned long long upto = mine;
+    const uint32_t batch = (uint32_t)p.batch, per = (batch + kThreads - 1) / kThreads;
+    const uint32_t b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+    uint32_t mine = 0;
+    for (uint32_t b = b0; b < b1; ++b) mine += R::units(tokens_of(p, b, blockIdx.x == 0));
+    uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long t = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
     if (lane == 31) warp_sum_s[warp] = upto;
     __syncthreads();
-    unsigned long long total = 0, before = 0;
+    uint32_t total = 0, before = 0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
         if (w == warp) before = total;
         total += warp_sum_s[w];
     }
-    before += upto - mine;  // pages of the sequences before b0
-    if (p.cum && cta == 0) {
-        unsigned long long c = before;
-        for (unsigned long long b = b0; b < b1; ++b) {
+    before += upto - mine;  // units (of one head) of the sequences before b0
+    if (p.cum && blockIdx.x == 0) {
+        uint32_t c = before;
+        for (uint32_t b = b0; b < b1; ++b) {
             p.cum[b] = c;
-            c += (tokens_of(p, b, false) + kPageTokens - 1) / kPageTokens;
+            c += R::units(tokens_of(p, b, false));
         }
-        if (tid == 0) p.cum[p.batch] = total;
+        if (tid == 0) p.cum[batch] = total;
     }
-    const unsigned long long units = total * p.v.heads;
-    *total_units = units;
-    Walker k{};
-    k.u = stretch_begin(units, cta, ctas);
-    k.end = stretch_begin(units, cta + 1, ctas);
-    if (k.u < k.end) {
-        const unsigned long long page = k.u / p.v.heads;  // the sequence whose pages hold this rank
-        if (page >= before && page < before + mine) {
-            unsigned long long b = b0, n, pages;
+    const Split ctas(total * p.v.heads, gridDim.x);
+    const uint32_t u0 = ctas.begin(blockIdx.x), u1 = ctas.begin(blockIdx.x + 1);
+    const Split parts(u1 - u0, kWarps);
+    *total_units = total * p.v.heads;
+    stretch[0] = u0;
+    stretch[1] = u1;
+    // (heads is a power of two)
+    const int shift = 31 - __clz(p.v.heads);
+    if (mine)
+        for (int w = 0; w < kWarps; ++w) {
+            const uint32_t a = u0 + parts.begin(w), rank = a >> shift;
+            if (a == u0 + parts.begin(w + 1) || rank < before || rank >= before + mine) continue;
+            uint32_t b = b0, c = before, n, k;
             while (true) {
                 n = tokens_of(p, b, false);
-                pages = (n + kPageTokens - 1) / kPageTokens;
-                if (page < before + pages) break;
-                before += pages;
+                k = R::units(n);
+                if (rank < c + k) break;
+                c += k;
                 ++b;
             }
-            found[0] = b;
-            found[1] = n;
-            found[2] = before;
+            found[w][0] = b;
+            found[w][1] = n;
+            found[w][2] = c;
         }
-    }
     __syncthreads();
-    if (k.u < k.end) {
-        k.seq = found[0];
-        k.tokens = found[1];
-        k.pages = (k.tokens + kPageTokens - 1) / kPageTokens;
-        const unsigned long long base = found[2] * p.v.heads;
-        k.head = (int)((k.u - base) / k.pages);
-        k.run = base + k.head * k.pages;
+    Walker<R> k{};
+    k.u = u0 + parts.begin(warp);
+    k.end = u0 + parts.begin(warp + 1);
+    if (!k.done()) {
+        k.seq = found[warp][0];
+        k.tokens = found[warp][1];
+        k.units = R::units(k.tokens);
+        const uint32_t base = found[warp][2] << shift;
+        k.head = (int)((k.u - base) / k.units);
+        k.run = base + k.head * k.units;
     }
     return k;
 }
+
+// A run's cut piece in a warp's part: [0] the run began before the part, [1] it goes on behind it.
+struct Piece {
+    uint32_t id, first, last;  // sequence * heads + head; its units [first, last)
+    int there, ends;           // ends: within the part
+};
 
 template <int F, typename Q, bool kFinal>
 __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(const __grid_constant__ PagedAttention p) {
     using Fmt = PageFormat<F>;
     using R = Ring<F>;
-    constexpr int kConsumers = R::kConsumers, kThreads = R::kThreads;
+    constexpr int kWarps = R::kWarps, kThreads = R::kThreads, kSlots = R::kSlots, kTiles = R::kTokens / 16;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[R::kStages], empty[R::kStages];
-    __shared__ int bad[R::kStages];
-    __shared__ volatile int dead;
-    unsigned char* ring = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
-    float* merge = reinterpret_cast<float*>(ring + R::kData);  // [warp][head][kOutPitch], then [warp][head][2]
-    float* merge_ml = merge + kConsumers * kGroup * kOutPitch;
+    __shared__ uint64_t full_s[kWarps][kSlots];
+    __shared__ int bad_s[kWarps][kSlots];
+    __shared__ Piece pieces[kWarps][2];
+    unsigned char* const ring0 = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) {
-        for (int s = 0; s < R::kStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 2);
-        }
+    float* const heads_s = reinterpret_cast<float*>(ring0 + kWarps * kSlots * R::kSlot);  // pieces [0]
+    unsigned char* const ring = ring0 + warp * kSlots * R::kSlot;
+    uint64_t* const full = full_s[warp];
+    int* const bad = bad_s[warp];
+    if (lane == 0) {
+        for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], 1);
         mbar_fence_init();
-        dead = 0;
+        pieces[warp][0].there = pieces[warp][1].there = 0;
     }
     pdl_wait();
     pdl_trigger();
-    unsigned long long units;
-    Walker k = find_stretch<kThreads>(p, blockIdx.x, gridDim.x, &units);  // syncs: the barriers are ready
+    uint32_t units, stretch[2];
+    Walker<R> k = find_part<R>(p, &units, stretch);  // syncs: the barriers are ready
     if (kFinal) {  // empty sequences: zeros
-        for (unsigned long long b = blockIdx.x; b < p.batch; b += gridDim.x)
+        for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
             if (tokens_of(p, b, false) == 0)
                 for (int i = tid; i < p.v.heads * kGroup * kDim; i += kThreads)
-                    p.out[b * p.v.heads * kGroup * kDim + i] = 0.0f;
+                    p.out[(size_t)b * p.v.heads * kGroup * kDim + i] = 0.0f;
     }
     if (tid == 0) {
         RunInfo info{};
         info.run = -1;
-        info.units = units;
         p.info[blockIdx.x] = info;
     }
-    if (k.u >= k.end) return;
-    const unsigned long long begin = k.u;
+    if (stretch[0] >= stretch[1]) return;
 
-    if (warp == kConsumers) {
-        // ---------------- producer: one block per unit
-        uint32_t it = 0;
-        bool ok = true;
-        for (; ok && k.u < k.end; k.next(p)) {
-            const unsigned long long stop = k.stop();
-            for (unsigned long long u = k.u; ok && u < stop; u += 32) {
-                const unsigned long long mine = u + lane;
-                const int32_t page = mine < stop ? p.v.table[k.seq * p.v.pitch + (mine - k.run)] : 0;
-                const int n = (int)min(stop - u, 32ull);
-                for (int i = 0; i < n; ++i, ++it) {
-                    const uint32_t s = it % R::kStages;
-                    if (it >= R::kStages) ok = mbar_wait(&empty[s], ((it / R::kStages) - 1) & 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const int32_t id = __shfl_sync(0xffffffffu, page, i);
-                    if (lane == 0) {
-                        const bool have = id >= 0 && (unsigned long long)id < p.v.pages;
-                        bad[s] = !have;
-                        if (have) {
-                            mbar_arrive_expect_tx(&full[s], Fmt::kBytes);
-                            bulk_copy_g2s(ring + s * Fmt::kBytes,
-                                          p.v.data + ((size_t)id * p.v.heads + k.head) * Fmt::kBytes, Fmt::kBytes,
-                                          &full[s]);
-                        } else {  // no such page: its tokens are left out
-                            raise_status(p.status, HSB_E_KV_PAGE, (int)k.seq);
-                            mbar_arrive(&full[s]);
-                        }
-                    }
-                }
+    // ---- feeding: K (even) or V (odd) of unit feed.u into slot fed % kSlots
+    Walker<R> feed = k;
+    uint32_t fed = 0, ids_first = 0;
+    int32_t ids = 0;  // table entries of 32 pages from ids_first
+    int32_t id = 0;
+    bool fresh = true;
+    const auto feed_one = [&]() {
+        const int s = fed % kSlots, part = fed & 1;
+        if (part == 0) {
+            const uint32_t page = (feed.u - feed.run) / R::kPerPage;
+            if (fresh || page >= ids_first + 32) {
+                ids_first = page;
+                ids = (page + lane) * R::kPerPage < feed.units ? p.v.table[feed.seq * p.v.pitch + page + lane] : 0;
+            }
+            id = __shfl_sync(0xffffffffu, ids, (int)(page - ids_first));
+        }
+        if (lane == 0) {
+            if (id >= 0 && (unsigned long long)id < p.v.pages) {
+                const int half = (int)((feed.u - feed.run) % R::kPerPage);
+                const unsigned char* src = p.v.data + ((size_t)id * p.v.heads + feed.head) * Fmt::kBytes;
+                unsigned char* dst = ring + s * R::kSlot;
+                bad[s] = 0;
+                mbar_arrive_expect_tx(&full[s], R::kSlot);
+#pragma unroll
+                for (int i = 0; i < Fmt::kPanels; ++i)
+                    bulk_copy_g2s(dst + i * R::kPanel, src + (part * Fmt::kPanels + i) * kPanelBytes + half * R::kPanel,
+                                  R::kPanel, &full[s]);
+                if constexpr (Fmt::kScaled)
+                    bulk_copy_g2s(dst + R::kScales, src + Fmt::kScaleOffset + part * kPageTokens * 4, kPageTokens * 4, &full[s]);
+            } else {  // no such page: its tokens are left out
+                if (part == 0) raise_status(p.status, HSB_E_KV_PAGE, (int)feed.seq);
+                bad[s] = 1;
+                mbar_arrive(&full[s]);
             }
         }
-        if (!ok) {  // give up, once the copies in flight have landed
-            if (lane == 0) {
-                raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
-                dead = 1;
-            }
-            const uint32_t first = it > R::kStages ? it - R::kStages : 0;
-            for (uint32_t j = first; j < it; ++j) (void)mbar_wait(&full[j % R::kStages], (j / R::kStages) & 1);
-        }
-        return;
-    }
+        if (part) fresh = feed.step(p);
+        ++fed;
+    };
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i)
+        if (!feed.done()) feed_one();
 
-    // ---------------- consumers
     const int g = lane >> 2, t = lane & 3;
-    const bool low = t >= 2;        // this lane's accumulator columns are the remainders' (and g >= 4 in B fragments)
-    const int h0 = 2 * (t & 1);     // they are heads h0 and h0 + 1 of the group
-    uint32_t hp0 = 0;               // half pages of the stretch before the current segment
-    for (; k.u < k.end; k.next(p)) {
-        const unsigned long long stop = k.stop();
-        const uint32_t hp1 = hp0 + 2 * (uint32_t)(stop - k.u);
-        float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f}, vref = 0.0f;
+    const bool low = t >= 2;     // this lane's accumulator columns are the remainders' (and g >= 4 in B fragments)
+    const int h0 = 2 * (t & 1);  // they are heads h0 and h0 + 1 of the group
+    // Of a unit's 8-token rows i (tokens 8 i + g), lanes t < 2 do the softmax of the first
+    // kTiles, lanes t >= 2 of the others; both have the same heads.
+    const int token0 = (low ? kTiles * 8 : 0) + g;
+    uint32_t it = 0;  // K and V parts read
+    bool alive = true;
+    while (alive && !k.done()) {
+        // ================ one run, as far as it lies in this part
+        const uint32_t begin = k.u, run_begin = k.run, run_end = k.run_end(), tokens = k.tokens;
+        const uint32_t stop = min(run_end, k.end), run = k.seq * p.v.heads + k.head;
+        float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f}, vref = 0.0f, vunit = Fmt::kScaled ? 0.0f : kWeightUnit;
         float o[8][4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        uint32_t hp = hp0 + (warp + kConsumers - hp0 % kConsumers) % kConsumers;
-        if (hp < hp1) {
-            // Q^T fragments: column g = head g & 3, its rounding or remainder (g >= 4)
-            uint32_t bq[8][2];
-            float sw[2];
-            {
-                const Q* q = static_cast<const Q*>(p.q) + ((k.seq * p.v.heads + k.head) * kGroup + (g & 3)) * kDim;
-                float x[8][4], top = 0.0f;
+        // Q^T fragments: column g = head g & 3, its rounding or remainder (g >= 4)
+        uint32_t bq[8][2];
+        float sw[2];
+        {
+            const Q* q = static_cast<const Q*>(p.q) + ((size_t)run * kGroup + (g & 3)) * kDim;
+            float4 x[8];
+            float top = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const int c = Fmt::kScaled ? t * 32 + ks * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
+            for (int ks = 0; ks < 8; ++ks)
+                x[ks] = load_q4(q + (Fmt::kScaled ? t * 32 + ks * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[ks][i] = load_q(q, c + i);
-                }
+            for (int ks = 0; ks < 8; ++ks)
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[ks].x), fabsf(x[ks].y)), fmaxf(fabsf(x[ks].z), fabsf(x[ks].w))));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // per head, 2^e brings max |q| into [2^14, 2^15): neither half leaves F16's normal range
+            const int qe = (int)((__float_as_uint(top) >> 23) & 0xffu);
+            const int e = (qe == 0 || qe == 0xff) ? 0 : max(-100, min(100, 141 - qe));
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[ks][i]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // per head, 2^e brings max |q| into [2^14, 2^15): neither half leaves F16's normal range
-                const int qe = (int)((__float_as_uint(top) >> 23) & 0xffu);
-                const int e = (qe == 0 || qe == 0xff) ? 0 : max(-100, min(100, 141 - qe));
-                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        bq[ks][i] = pack2(split_half(x[ks][2 * i] * up, g >= 4), split_half(x[ks][2 * i + 1] * up, g >= 4));
-                const float s = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
-                sw[0] = __shfl_sync(0xffffffffu, s, h0 * 4);
-                sw[1] = __shfl_sync(0xffffffffu, s, (h0 + 1) * 4);
+            for (int ks = 0; ks < 8; ++ks) {
+                bq[ks][0] = split_pair(x[ks].x * up, x[ks].y * up, g >= 4);
+                bq[ks][1] = split_pair(x[ks].z * up, x[ks].w * up, g >= 4);
             }
-            for (; hp < hp1; hp += kConsumers) {
-                const uint32_t unit = hp >> 1;  // of the stretch
-                const uint32_t s = unit % R::kStages;
-                if (!__all_sync(0xffffffffu, !dead && mbar_wait(&full[s], (unit / R::kStages) & 1))) {
-                    if (lane == 0) {
-                        raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
-                        dead = 1;
-                    }
-                    break;
-                }
-                const int r0 = (int)(hp & 1) * 32;
-                const unsigned long long at = (begin + unit - k.run) * kPageTokens + r0;
-                const int live = bad[s] || at >= k.tokens ? 0 : (int)min(k.tokens - at, 32ull);
-                if (live) {
-                    const uint32_t blk = smem_addr(ring + s * Fmt::kBytes);
-                    // ---- logits
-                    float acc[2][4];
+            const float s = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+            sw[0] = __shfl_sync(0xffffffffu, s, h0 * 4);
+            sw[1] = __shfl_sync(0xffffffffu, s, (h0 + 1) * 4);
+        }
+        for (uint32_t u = begin; u < stop; ++u) {
+            const int live = (int)min(tokens - (u - run_begin) * R::kTokens, (uint32_t)R::kTokens);
+            // ---------------- K: logits
+            uint32_t s = it % kSlots;
+            alive = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kSlots) & 1));
+            if (!alive) break;
+            const bool skip = bad[s];
+            uint32_t blk = smem_addr(ring + s * R::kSlot);
+            float x[2][kTiles];  // [head][own row]
+            {
+                float acc[kTiles][4];
 #pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
-                        acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.0f;
-                        const uint32_t ra = blk + (r0 + mt * 16 + g) * 128;
+                for (int mt = 0; mt < kTiles; ++mt) {
+                    acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.0f;
+                    const uint32_t ra = blk + (mt * 16 + g) * 128;
 #pragma unroll
-                        for (int pl = 0; pl < Fmt::kPanels; ++pl)
+                    for (int pl = 0; pl < Fmt::kPanels; ++pl)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t at16 = ra + pl * kPanelBytes + (((2 * t + i) ^ g) << 4);
-                                const uint4 va = lds128(at16), vb = lds128(at16 + 8 * 128);
-                                const uint32_t a[4] = {va.x, va.y, va.z, va.w}, b[4] = {vb.x, vb.y, vb.z, vb.w};
-                                if constexpr (Fmt::kScaled) {
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t at16 = ra + pl * R::kPanel + (((2 * t + i) ^ g) << 4);
+                            const uint4 va = lds128(at16), vb = lds128(at16 + 8 * 128);
+                            const uint32_t a[4] = {va.x, va.y, va.z, va.w}, b[4] = {vb.x, vb.y, vb.z, vb.w};
+                            if constexpr (Fmt::kScaled) {
 #pragma unroll
-                                    for (int w = 0; w < 4; ++w) {
-                                        uint32_t a0, a2, a1, a3;
-                                        codes_to_half2<F>(a[w], a0, a2);
-                                        codes_to_half2<F>(b[w], a1, a3);
-                                        mma_f16(acc[mt], a0, a1, a2, a3, bq[i * 4 + w][0], bq[i * 4 + w][1]);
-                                    }
-                                } else {
+                                for (int w = 0; w < 4; ++w) {
+                                    uint32_t a0, a2, a1, a3;
+                                    codes_to_half2<F>(a[w], a0, a2);
+                                    codes_to_half2<F>(b[w], a1, a3);
+                                    mma_f16(acc[mt], a0, a1, a2, a3, bq[i * 4 + w][0], bq[i * 4 + w][1]);
+                                }
+                            } else {
 #pragma unroll
-                                    for (int w = 0; w < 2; ++w) {
-                                        const int ks = pl * 4 + i * 2 + w;
-                                        mma_f16(acc[mt], a[2 * w], b[2 * w], a[2 * w + 1], b[2 * w + 1], bq[ks][0], bq[ks][1]);
-                                    }
+                                for (int w = 0; w < 2; ++w) {
+                                    const int ks = pl * 4 + i * 2 + w;
+                                    mma_f16(acc[mt], a[2 * w], b[2 * w], a[2 * w + 1], b[2 * w + 1], bq[ks][0], bq[ks][1]);
                                 }
                             }
-                    }
-                    // ---- online softmax: this lane has tokens g + 8 i of heads h0, h0 + 1
-                    float vs[4] = {kWeightTop, kWeightTop, kWeightTop, kWeightTop};
-                    float x[2][4];  // [head][i]
-                    float vfold = 1.0f;
-                    if constexpr (Fmt::kScaled) {
-                        const uint32_t sc = blk + Fmt::kScaleOffset + (r0 + g) * 4;
-                        float vtop = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            vs[i] = lds32(sc + kPageTokens * 4 + i * 32);
-                            if (8 * i + g < live) vtop = fmaxf(vtop, vs[i]);
                         }
-                        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 4));
-                        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 8));
-                        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 16));
-                        // the next power of two: weight x scale stays within kWeightTop
-                        const float up = __uint_as_float((__float_as_uint(vtop) + 0x7fffffu) & 0xff800000u);
+                }
+                // rounding + remainder: each lane gives away the rows it does not own
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float a = acc[e >> 1][(e & 1) * 2 + j], b = acc[(kTiles + e) >> 1][(e & 1) * 2 + j];
+                        x[j][e] = (low ? b : a) + __shfl_xor_sync(0xffffffffu, low ? a : b, 2);
+                    }
+            }
+            if constexpr (Fmt::kScaled) {
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e) {
+                    const float ks = lds32(blk + R::kScales + (token0 + 8 * e) * 4);
+                    x[0][e] *= sw[0] * ks;
+                    x[1][e] *= sw[1] * ks;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e) {
+                    x[0][e] *= sw[0];
+                    x[1][e] *= sw[1];
+                }
+            }
+            __syncwarp();  // the slot is read
+            if (!feed.done()) feed_one();
+            ++it;
+            // ---------------- V: weights and output
+            s = it % kSlots;
+            alive = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kSlots) & 1));
+            if (!alive) break;
+            if (!skip) {
+                blk = smem_addr(ring + s * R::kSlot);
+                float vs[kTiles];
+                if constexpr (Fmt::kScaled) {
+#pragma unroll
+                    for (int e = 0; e < kTiles; ++e) vs[e] = lds32(blk + R::kScales + (token0 + 8 * e) * 4);
+                }
+                if (live < R::kTokens) {
+#pragma unroll
+                    for (int e = 0; e < kTiles; ++e)
+                        if (token0 + 8 * e >= live) {
+                            x[0][e] = x[1][e] = -INFINITY;
+                            vs[e] = 0.0f;  // an unwritten row's scale may be anything
+                        }
+                }
+                bool grown = false;
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e) {
+                    grown |= x[0][e] > M[0] + kSlack || x[1][e] > M[1] + kSlack;
+                    if constexpr (Fmt::kScaled) grown |= vs[e] > vref;
+                }
+                if (__any_sync(0xffffffffu, grown)) {
+                    // move the maxima (of both lanes' rows) and the power of two over the V scales
+                    float fold[2], vfold = 1.0f;
+                    if constexpr (Fmt::kScaled) {
+                        float top = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < kTiles; ++e) top = fmaxf(top, vs[e]);
+                        top = warp_max(top);
+                        const float up = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0xff800000u);
                         if (up > vref) {
                             vfold = vref / up;
                             vref = up;
-                        }
-                        const float inv = vref > 0.0f ? kWeightTop / vref : 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) vs[i] *= inv;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float ks = lds32(sc + i * 32);
-                            const int mt = i >> 1, r = (i & 1) * 2;
-                            x[0][i] = (acc[mt][r] + __shfl_xor_sync(0xffffffffu, acc[mt][r], 2)) * (sw[0] * ks);
-                            x[1][i] = (acc[mt][r + 1] + __shfl_xor_sync(0xffffffffu, acc[mt][r + 1], 2)) * (sw[1] * ks);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int mt = i >> 1, r = (i & 1) * 2;
-                            x[0][i] = (acc[mt][r] + __shfl_xor_sync(0xffffffffu, acc[mt][r], 2)) * sw[0];
-                            x[1][i] = (acc[mt][r + 1] + __shfl_xor_sync(0xffffffffu, acc[mt][r + 1], 2)) * sw[1];
+                            vunit = kWeightUnit / up;
                         }
                     }
-                    if (live < 32) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (8 * i + g >= live) {
-                                x[0][i] = x[1][i] = -INFINITY;
-                                vs[i] = 0.0f;  // an unwritten row's scale may be anything
-                            }
-                    }
-                    float mx[2], fold[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        mx[j] = fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3]));
-                        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
-                        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
-                        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
-                        mx[j] = fmaxf(M[j], mx[j]);
-                    }
-                    // the accumulators change scale only where a maximum (or the V reference) grew
-                    if (__any_sync(0xffffffffu, mx[0] > M[0] || mx[1] > M[1] || vfold != 1.0f)) {
+                        float top = x[j][0];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            fold[j] = M[j] == -INFINITY ? 0.0f : exp2f(M[j] - mx[j]);
-                            L[j] *= fold[j];
-                            fold[j] *= vfold;
-                            M[j] = mx[j];
+                        for (int e = 1; e < kTiles; ++e) top = fmaxf(top, x[j][e]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, M[j]);
+                        fold[j] = M[j] == -INFINITY ? 0.0f : exp2_ftz(M[j] - top);
+                        L[j] *= fold[j];
+                        fold[j] *= vfold;
+                        M[j] = top;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[j][0] *= fold[0];
+                        o[j][1] *= fold[1];
+                        o[j][2] *= fold[0];
+                        o[j][3] *= fold[1];
+                    }
+                }
+                const float base0 = M[0] == -INFINITY ? 0.0f : M[0], base1 = M[1] == -INFINITY ? 0.0f : M[1];
+                uint32_t bp[2 * kTiles];  // P^T fragments of rows i
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e) {
+                    const float p0 = exp2_ftz(x[0][e] - base0), p1 = exp2_ftz(x[1][e] - base1);
+                    L[0] += p0;
+                    L[1] += p1;
+                    const float unit = Fmt::kScaled ? vs[e] * vunit : kWeightUnit;
+                    const __half2 hi = __floats2half2_rn(p0 * unit, p1 * unit);
+                    const float2 f = __half22float2(hi);
+                    const __half2 lo = __floats2half2_rn(p0 * unit - f.x, p1 * unit - f.y);
+                    const uint32_t hw = *reinterpret_cast<const uint32_t*>(&hi), lw = *reinterpret_cast<const uint32_t*>(&lo);
+                    const uint32_t keep = low ? lw : hw, other = __shfl_xor_sync(0xffffffffu, low ? hw : lw, 2);
+                    bp[e] = transpose_8x8(low ? other : keep);
+                    bp[kTiles + e] = transpose_8x8(low ? keep : other);
+                }
+#pragma unroll
+                for (int kt = 0; kt < kTiles; ++kt) {
+                    const int row = kt * 16 + 2 * t;  // and + 1, + 8, + 9
+                    const uint32_t ra = blk + row * 128;
+#pragma unroll
+                    for (int pl = 0; pl < Fmt::kPanels; ++pl) {
+                        uint4 v[4];
+                        v[0] = lds128(ra + pl * R::kPanel + ((g ^ (2 * t)) << 4));
+                        v[1] = lds128(ra + pl * R::kPanel + 128 + ((g ^ (2 * t + 1)) << 4));
+                        v[2] = lds128(ra + pl * R::kPanel + 8 * 128 + ((g ^ (2 * t)) << 4));
+                        v[3] = lds128(ra + pl * R::kPanel + 9 * 128 + ((g ^ (2 * t + 1)) << 4));
+                        if (live < R::kTokens) {  // rows behind the last token may hold NaN: 0 x NaN must not enter
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (row + (i >> 1) * 8 + (i & 1) >= live) v[i] = make_uint4(0, 0, 0, 0);
                         }
+                        const uint32_t A[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, B[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+                        const uint32_t C[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, D[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            o[j][0] *= fold[0];
-                            o[j][1] *= fold[1];
-                            o[j][2] *= fold[0];
-                            o[j][3] *= fold[1];
-                        }
-                    }
-                    const float base0 = M[0] == -INFINITY ? 0.0f : M[0], base1 = M[1] == -INFINITY ? 0.0f : M[1];
-                    uint32_t bp[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p0 = exp2f(x[0][i] - base0), p1 = exp2f(x[1][i] - base1);
-                        L[0] += p0;
-                        L[1] += p1;
-                        bp[i] = transpose_8x8(pack2(split_half(p0 * vs[i], low), split_half(p1 * vs[i], low)));
-                    }
-                    // ---- output
-                    const uint32_t vb = blk + Fmt::kPanels * kPanelBytes;
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        const int row = kt * 16 + 2 * t;  // and + 1, + 8, + 9
-                        const uint32_t ra = vb + (r0 + row) * 128;
-#pragma unroll
-                        for (int pl = 0; pl < Fmt::kPanels; ++pl) {
-                            uint4 v[4];
-                            v[0] = lds128(ra + pl * kPanelBytes + ((g ^ (2 * t)) << 4));
-                            v[1] = lds128(ra + pl * kPanelBytes + 128 + ((g ^ (2 * t + 1)) << 4));
-                            v[2] = lds128(ra + pl * kPanelBytes + 8 * 128 + ((g ^ (2 * t)) << 4));
-                            v[3] = lds128(ra + pl * kPanelBytes + 9 * 128 + ((g ^ (2 * t + 1)) << 4));
-                            if (live < 32) {  // rows behind the last token may hold NaN: 0 x NaN must not enter
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (row + (i >> 1) * 8 + (i & 1) >= live) v[i] = make_uint4(0, 0, 0, 0);
-                            }
-                            const uint32_t A[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, B[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-                            const uint32_t C[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, D[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                if constexpr (Fmt::kScaled) {
-                                    // bytes of two tokens interleaved: channel by channel (token, token + 1)
-                                    uint32_t a0, a1, a2, a3;
-                                    codes_to_half2<F>(__byte_perm(A[w], B[w], 0x5140), a0, a1);
-                                    codes_to_half2<F>(__byte_perm(C[w], D[w], 0x5140), a2, a3);
-                                    mma_f16(o[2 * w], a0, a1, a2, a3, bp[2 * kt], bp[2 * kt + 1]);
-                                    codes_to_half2<F>(__byte_perm(A[w], B[w], 0x7362), a0, a1);
-                                    codes_to_half2<F>(__byte_perm(C[w], D[w], 0x7362), a2, a3);
-                                    mma_f16(o[2 * w + 1], a0, a1, a2, a3, bp[2 * kt], bp[2 * kt + 1]);
-                                } else {
-                                    mma_f16(o[pl * 4 + w], __byte_perm(A[w], B[w], 0x5410), __byte_perm(A[w], B[w], 0x7632),
-                                            __byte_perm(C[w], D[w], 0x5410), __byte_perm(C[w], D[w], 0x7632), bp[2 * kt],
-                                            bp[2 * kt + 1]);
-                                }
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (Fmt::kScaled) {
+                                // bytes of two tokens interleaved: channel by channel (token, token + 1)
+                                uint32_t a0, a1, a2, a3;
+                                codes_to_half2<F>(__byte_perm(A[w], B[w], 0x5140), a0, a1);
+                                codes_to_half2<F>(__byte_perm(C[w], D[w], 0x5140), a2, a3);
+                                mma_f16(o[2 * w], a0, a1, a2, a3, bp[2 * kt], bp[2 * kt + 1]);
+                                codes_to_half2<F>(__byte_perm(A[w], B[w], 0x7362), a0, a1);
+                                codes_to_half2<F>(__byte_perm(C[w], D[w], 0x7362), a2, a3);
+                                mma_f16(o[2 * w + 1], a0, a1, a2, a3, bp[2 * kt], bp[2 * kt + 1]);
+                            } else {
+                                mma_f16(o[pl * 4 + w], __byte_perm(A[w], B[w], 0x5410), __byte_perm(A[w], B[w], 0x7632),
+                                        __byte_perm(C[w], D[w], 0x5410), __byte_perm(C[w], D[w], 0x7632), bp[2 * kt],
+                                        bp[2 * kt + 1]);
                             }
                         }
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
             }
+            __syncwarp();
+            if (!feed.done()) feed_one();
+            ++it;
         }
-        // ---- the segment's end: rounding + remainder, then the warps together
-        const float os = Fmt::kScaled ? vref / kWeightTop : 1.0f / kWeightTop;
+        if (!alive) break;
+        // ---------------- the run's end here: all rows' sums, rounding + remainder
+        const float os = Fmt::kScaled ? vref / kWeightUnit : 1.0f / kWeightUnit;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+            L[j] += __shfl_xor_sync(0xffffffffu, L[j], 2);
             L[j] += __shfl_xor_sync(0xffffffffu, L[j], 4);
             L[j] += __shfl_xor_sync(0xffffffffu, L[j], 8);
             L[j] += __shfl_xor_sync(0xffffffffu, L[j], 16);
@@ -495,66 +551,110 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[j][r] = (o[j][r] + __shfl_xor_sync(0xffffffffu, o[j][r], 2)) * os;
+        const bool begins = run_begin >= begin, ends = run_end <= k.end, whole = begins && ends;
+        if (!whole && lane == 0) {
+            Piece& c = pieces[warp][begins];
+            c.id = run;
+            c.first = run_begin;
+            c.last = run_end;
+            c.ends = ends;
+            c.there = 1;
+        }
+        float* slot = whole ? p.whole + (size_t)run * kPartFloats
+                            : begins ? reinterpret_cast<float*>(ring) : heads_s + warp * kPartFloats;
         if (!low) {
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-                const int slot = warp * kGroup + h0 + hh;
-                if (g == 0) {
-                    merge_ml[slot * 2] = M[hh];
-                    merge_ml[slot * 2 + 1] = L[hh];
+                const float inv = L[hh] > 0.0f ? 1.0f / L[hh] : (L[hh] == L[hh] ? 0.0f : L[hh]);
+                const bool final = kFinal && whole;
+                float* dst = final ? p.out + ((size_t)run * kGroup + h0 + hh) * kDim : slot + 2 * kGroup + (h0 + hh) * kDim;
+                if (!final && g == 0) {
+                    slot[2 * (h0 + hh)] = M[hh];
+                    slot[2 * (h0 + hh) + 1] = L[hh];
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {  // MMA rows g, g + 8 of tile j: two neighbouring channels
                     const int c = Fmt::kScaled ? g * 16 + 2 * j : (j >> 2) * 64 + g * 8 + (j & 3) * 2;
-                    *reinterpret_cast<float2*>(merge + slot * kOutPitch + c) = make_float2(o[j][hh], o[j][hh + 2]);
+                    *reinterpret_cast<float2*>(dst + c) =
+                        final ? make_float2(o[j][hh] * inv, o[j][hh + 2] * inv) : make_float2(o[j][hh], o[j][hh + 2]);
                 }
             }
         }
-        named_sync(1, kConsumers * 32);
-        for (int i = tid; i < kGroup * kDim / 2; i += kConsumers * 32) {
-            const int h = i >> 6, c = (i & 63) * 2;
+        k.u = stop - 1;  // to the next run
+        k.step(p);
+    }
+    if (!alive) {  // gave up: copies in flight land before shared memory is released
+        if (lane == 0) raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
+        for (uint32_t j = it; j < fed; ++j) (void)mbar_wait(&full[j % kSlots], (j / kSlots) & 1);
+    }
+    __syncthreads();
+    // ================ the runs that crossed warps: pieces of one run, in order
+    const auto piece_at = [&](int w, int which) -> const float* {
+        return which ? reinterpret_cast<const float*>(ring0 + w * kSlots * R::kSlot) : heads_s + w * kPartFloats;
+    };
+    const auto fold_run = [&](int w0, int which, int w1) {
+        const Piece& c = pieces[w0][which];
+        const bool begins = c.first >= stretch[0], ends = c.last <= stretch[1];
+        for (int i = tid; i < kGroup * kDim / 2; i += kThreads) {
+            const int h = i >> 6, at = 2 * kGroup + i * 2;
             float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kConsumers; ++w) top = fmaxf(top, merge_ml[(w * kGroup + h) * 2]);
+            for (int w = w0; w <= w1; ++w)
+                if (w == w0 || pieces[w][0].there) top = fmaxf(top, piece_at(w, w == w0 && which)[2 * h]);
             float sum = 0.0f, a = 0.0f, b = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kConsumers; ++w) {
-                // (a warp without tokens has sum 0; a NaN sum must come through)
-                const float f = top == -INFINITY ? 1.0f : exp2f(merge_ml[(w * kGroup + h) * 2] - top);
-                const float2 v = *reinterpret_cast<const float2*>(merge + (w * kGroup + h) * kOutPitch + c);
-                sum = fmaf(f, merge_ml[(w * kGroup + h) * 2 + 1], sum);
+            for (int w = w0; w <= w1; ++w) {
+                if (w != w0 && !pieces[w][0].there) continue;
+                const float* part = piece_at(w, w == w0 && which);
+                // (no token under a finite maximum: sum 0; a NaN sum comes through)
+                const float f = top == -INFINITY ? 1.0f : exp2f(part[2 * h] - top);
+                const float2 v = *reinterpret_cast<const float2*>(part + at);
+                sum = fmaf(f, part[2 * h + 1], sum);
                 a = fmaf(f, v.x, a);
                 b = fmaf(f, v.y, b);
             }
-            const bool begins = k.run >= begin, ends = k.run + k.pages <= k.end;
-            const unsigned long long run = k.seq * p.v.heads + k.head;
             if (kFinal && begins && ends) {
                 const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
-                *reinterpret_cast<float2*>(p.out + (run * kGroup + h) * kDim + c) = make_float2(a * inv, b * inv);
+                *reinterpret_cast<float2*>(p.out + (size_t)c.id * kGroup * kDim + i * 2) = make_float2(a * inv, b * inv);
             } else {
-                float* slot = begins && ends ? p.whole + run * kPartFloats
-                                             : p.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kPartFloats;
-                *reinterpret_cast<float2*>(slot + 2 * kGroup + h * kDim + c) = make_float2(a, b);
-                if (c == 0) {
+                float* slot = begins && ends ? p.whole + (size_t)c.id * kPartFloats
+                                             : p.part + ((size_t)blockIdx.x * 2 + begins) * kPartFloats;
+                *reinterpret_cast<float2*>(slot + at) = make_float2(a, b);
+                if ((i & 63) == 0) {
                     slot[2 * h] = top;
                     slot[2 * h + 1] = sum;
                 }
-                if (i == 0 && begins && !ends) {
-                    RunInfo info{};
-                    info.run = (long long)run;
-                    info.units = units;
-                    info.last = stretch_of(units, k.run + k.pages - 1, gridDim.x);
-                    p.info[blockIdx.x] = info;
-                }
             }
         }
-        named_sync(1, kConsumers * 32);  // before the next segment writes the merge area
-        hp0 = hp1;
+        if (tid == 0 && begins && !ends) {
+            RunInfo info{};
+            info.run = (int)c.id;
+            info.last = Split(units, gridDim.x).of(c.last - 1);
+            p.info[blockIdx.x] = info;
+        }
+    };
+    int open = -1, which = 0, last = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (pieces[w][0].there) {
+            if (open < 0) {
+                open = w;
+                which = 0;
+            }
+            last = w;
+            if (pieces[w][0].ends) {
+                fold_run(open, which, w);
+                open = -1;
+            }
+        }
+        if (pieces[w][1].there) {
+            open = last = w;
+            which = 1;
+        }
     }
+    if (open >= 0) fold_run(open, which, last);
 }
 
 // Folds the partials of the run that begins in CTA blockIdx.x's stretch and
-// does not end there, in the order of the CTAs.  Thread = (head, channel).
+// does not end there, in the order of the CTAs (a run that goes on leaves no
+// empty stretch before its end).  Thread = (head, channel).
 __global__ void __launch_bounds__(kGroup* kDim) kv_combine_kernel(const float* __restrict__ part,
                                                                  const RunInfo* __restrict__ infos,
                                                                  float* __restrict__ out) {
@@ -565,37 +665,38 @@ __global__ void __launch_bounds__(kGroup* kDim) kv_combine_kernel(const float* _
     const RunInfo info = infos[blockIdx.x];
     if (info.run < 0) return;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned first = blockIdx.x, ctas = gridDim.x;
-    const int n = (int)(info.last - first) + 1;
+    const int n = (int)(info.last - blockIdx.x) + 1;
+    // the first partial is its CTA's [1], the others their CTAs' [0]
+    const float* base = part + (size_t)blockIdx.x * 2 * kPartFloats;
+    const auto at = [&](int i) { return base + ((size_t)i * 2 + (i == 0)) * kPartFloats; };
     if (warp < kGroup) {  // weights of the partials of head `warp`
         float top = -INFINITY;
         for (int i = lane; i < n; i += 32) {
-            const unsigned c = first + i;
-            const bool some = stretch_begin(info.units, c, ctas) < stretch_begin(info.units, c + 1, ctas);
-            const float m = some ? part[((size_t)c * 2 + (i == 0)) * kPartFloats + 2 * warp] : INFINITY;
+            const float m = __ldcg(at(i) + 2 * warp);
             weight[warp][i] = m;
-            if (some) top = fmaxf(top, m);
+            top = fmaxf(top, m);
         }
         top = warp_max(top);
         float sum = 0.0f;
         for (int i = lane; i < n; i += 32) {
-            const float m = weight[warp][i];
-            // -1: an empty stretch, which left nothing
-            const float f = m == INFINITY ? -1.0f : top == -INFINITY ? 1.0f : exp2f(m - top);
+            const float f = top == -INFINITY ? 1.0f : exp2f(weight[warp][i] - top);
             weight[warp][i] = f;
-            if (f >= 0.0f) sum = fmaf(f, part[((size_t)(first + i) * 2 + (i == 0)) * kPartFloats + 2 * warp + 1], sum);
+            sum = fmaf(f, __ldcg(at(i) + 2 * warp + 1), sum);
         }
         sum = warp_sum(sum);
         if (lane == 0) inv[warp] = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
     }
+    float first[8];  // the first outputs are on their way meanwhile
+#pragma unroll
+    for (int i = 0; i < 8; ++i) first[i] = i < n ? __ldcg(at(i) + 2 * kGroup + tid) : 0.0f;
     __syncthreads();
     const int h = tid / kDim;
     float acc = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) acc = fmaf(weight[h][i], first[i], acc);
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-        const float f = weight[h][i];
-        if (f >= 0.0f) acc = fmaf(f, part[((size_t)(first + i) * 2 + (i == 0)) * kPartFloats + 2 * kGroup + tid], acc);
-    }
+    for (int i = 8; i < n; ++i) acc = fmaf(weight[h][i], __ldcg(at(i) + 2 * kGroup + tid), acc);
     out[(size_t)info.run * kGroup * kDim + tid] = acc * inv[h];
 }
 
@@ -651,7 +752,7 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     if (!d_table || !table_width || table_width > kMaxTableEntries || !d_lengths || !batch || batch > kMaxBatch ||
         batch * table_width > kMaxTableEntries || !d_q || !d_out)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
-    if ((reinterpret_cast<uintptr_t>(d_q) & 3u) || (reinterpret_cast<uintptr_t>(d_out) & 7u) ||
+    if ((reinterpret_cast<uintptr_t>(d_q) & 15u) || (reinterpret_cast<uintptr_t>(d_out) & 7u) ||
         (reinterpret_cast<uintptr_t>(d_workspace) & 15u))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
     if (!d_workspace || workspace_bytes < hsb_kv_attention_workspace_bytes(batch, pages->kv_heads))

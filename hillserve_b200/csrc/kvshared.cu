@@ -10,14 +10,14 @@ namespace {
 struct Source {
     const float* part;
     const float* whole;
-    unsigned long long units;
+    uint32_t units;
     unsigned ctas;
 };
 
 struct SharedCombine {
     Source prefix, own;
-    unsigned long long prefix_pages;
-    const unsigned long long* cum;
+    uint32_t prefix_units;
+    const uint32_t* cum;
     unsigned long long batch;
     int heads;
     uint16_t* out;
@@ -26,9 +26,9 @@ struct SharedCombine {
 __device__ __forceinline__ void fold(const Source& s, unsigned long long run, unsigned long long begin,
                                      unsigned long long pages, int h, int d, float& M, float& L, float& acc) {
     if (!pages) return;
-    const unsigned first = stretch_of(s.units, begin, s.ctas), last = stretch_of(s.units, begin + pages - 1, s.ctas);
+    const Split split(s.units, s.ctas);
+    const unsigned first = split.of((uint32_t)begin), last = split.of((uint32_t)(begin + pages - 1));
     for (unsigned c = first; c <= last; ++c) {
-        if (stretch_begin(s.units, c, s.ctas) == stretch_begin(s.units, c + 1, s.ctas)) continue;
         const float* slot = first == last ? s.whole + run * kPartFloats
                                           : s.part + ((size_t)c * 2 + (c == first)) * kPartFloats;
         const float m = __ldcg(slot + 2 * h), l = __ldcg(slot + 2 * h + 1);
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kGroup* kDim) kv_shared_combine_kernel(const _
     const int head = (int)(run % p.heads), h = threadIdx.x / kDim, d = threadIdx.x % kDim;
     float M = -INFINITY, L = 0.0f, acc = 0.0f;
     Source p_own = p.own;
-    fold(p.prefix, run, run * p.prefix_pages, p.prefix_pages, h, d, M, L, acc);
+    fold(p.prefix, run, run * p.prefix_units, p.prefix_units, h, d, M, L, acc);
     const unsigned long long pages = p.cum[seq + 1] - p.cum[seq];
     p_own.units = p.cum[p.batch] * p.heads;
     fold(p_own, run, p.cum[seq] * p.heads + head * pages, pages, h, d, M, L, acc);
@@ -108,23 +108,23 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
         p.length = prefix_tokens;
         p.batch = batch;
         p.q = d_q;
-        p.cum = reinterpret_cast<unsigned long long*>(ws);
+        p.cum = reinterpret_cast<uint32_t*>(ws);
         p.info = reinterpret_cast<RunInfo*>(ws + l.info);
         p.part = reinterpret_cast<float*>(ws + l.part);
         p.whole = reinterpret_cast<float*>(ws + l.whole);
         p.status = d_status;
         p.scale_log2 = kScaleLog2;
-        const unsigned grid = paged_attention_grid(batch * pages->kv_heads * p.v.width);
+        const unsigned grid = paged_attention_grid(2 * batch * pages->kv_heads * p.v.width);
         cudaError_t e = launch_paged_partials(which ? pages->format : HSB_KV_F16, p, grid, s);
         if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
         Source& src = which ? c.own : c.prefix;
         src.part = p.part;
         src.whole = p.whole;
-        src.units = which ? 0 : batch * pages->kv_heads * prefix_pages;
+        src.units = which ? 0 : batch * pages->kv_heads * ((prefix_tokens + 31) / 32);
         src.ctas = grid;
         c.cum = p.cum;
     }
-    c.prefix_pages = prefix_pages;
+    c.prefix_units = (prefix_tokens + 31) / 32;
     c.batch = batch;
     c.heads = pages->kv_heads;
     c.out = d_out;

@@ -105,7 +105,7 @@ def test_attention_refusals(lib):
     size = lib.hsb_kv_attention_workspace_bytes(2, 8)
     good = dict(pages=pool(), table=P, width=4, lengths=P, batch=2, q=P, out=P, ws=P, size=size, status=None, stream=None)
     for change in (dict(table=None), dict(width=0), dict(lengths=None), dict(batch=0), dict(batch=(1 << 20) + 1),
-                   dict(q=None), dict(out=None), dict(width=1 << 32), dict(width=1 << 31, batch=2),
+                   dict(q=None), dict(out=None), dict(width=1 << 32), dict(width=1 << 27, batch=2),
                    dict(q=C.c_void_p(0x10002)), dict(out=C.c_void_p(0x10004)), dict(ws=C.c_void_p(0x10008))):
         assert call(lib, "hsb_kv_attention", good, **change) == 120, change
     assert call(lib, "hsb_kv_attention", good, size=size - 1) == 3
@@ -129,22 +129,29 @@ def test_messages(lib):
         assert lib.hsb_status_message(code).startswith(b"paged KV ")
 
 
-def stretch_begin(units, c, n):
-    return units * c // n
+class Split:
+    """The even split of kvattention.cuh, restated."""
 
+    def __init__(self, units, n):
+        self.each, self.more = units // n, units % n
 
-def stretch_of(units, u, n):
-    return ((u + 1) * n + units - 1) // units - 1
+    def begin(self, c):
+        return self.each * c + min(c, self.more)
+
+    def of(self, u):
+        longer = (self.each + 1) * self.more
+        return u // (self.each + 1) if u < longer else self.more + (u - longer) // self.each
 
 
 @pytest.mark.parametrize("units", [1, 2, 7, 147, 148, 149, 1000, 4096 * 8 + 3])
 @pytest.mark.parametrize("n", [1, 2, 16, 148])
 def test_every_unit_has_the_stretch_that_holds_it(units, n):
-    """The split's two formulas (kvattention.cuh) agree: a run's folder finds its parts."""
+    """The split's two formulas agree, so a run's folder finds its parts; empty stretches are the last ones."""
+    s = Split(units, n)
     for u in {0, units - 1, units // 2, units // 3, min(units - 1, 5)}:
-        c = stretch_of(units, u, n)
-        assert 0 <= c < n and stretch_begin(units, c, n) <= u < stretch_begin(units, c + 1, n)
-    assert stretch_begin(units, n, n) == units
+        assert 0 <= s.of(u) < n and s.begin(s.of(u)) <= u < s.begin(s.of(u) + 1)
+    sizes = [s.begin(c + 1) - s.begin(c) for c in range(n)]
+    assert s.begin(n) == units and sizes == sorted(sizes, reverse=True) and sizes[0] - sizes[-1] <= 1
 
 
 def test_mirror_refusals():
