@@ -743,9 +743,10 @@ class KVPages:
         if data.device.type != "cuda":
             raise InvalidArgument(120, "a paged KV pool is CUDA device memory")
         self.data, self.pages, self.device = data, int(data.shape[0]), data.device
+        self._index, self._lib = data.get_device(), lib()
         self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
         self._c = KvPages(data.data_ptr(), self.pages, self.FORMATS[format], self.kv_heads)
-        self._ref, self._st = C.byref(self._c), C.c_void_p(self.status.data_ptr())
+        self._ref, self._st = C.byref(self._c), self.status.data_ptr()
 
     def check(self, stream=None) -> None:
         """Synchronises; raises (and forgets) what the calls so far recorded."""
@@ -756,30 +757,28 @@ class KVPages:
             self.status.zero_()
             raise
 
-    def _arg(self, t, name: str, dtypes: tuple, shape: tuple) -> int:
-        """Address of a contiguous tensor on the pool's device; -1 in shape: any extent."""
-        if t.device != self.device:
+    def _arg(self, t, name: str, dtype, shape: tuple) -> int:
+        """Address of a contiguous tensor of this type and shape on the pool's device."""
+        if t.dtype is dtype and t.shape == shape and t.get_device() == self._index and t.is_contiguous():
+            return t.data_ptr()
+        if t.get_device() != self._index:
             raise InvalidArgument(120, f"{name} must be on the pool's device, {self.device}")
-        if t.dtype not in dtypes:
-            raise InvalidArgument(120, f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, not {str(t.dtype)[6:]}")
-        if t.dim() != len(shape) or any(w not in (-1, n) for w, n in zip(shape, t.shape)) or not t.is_contiguous():
-            raise InvalidArgument(120, f"{name} must be {list(shape)}, contiguous; got {list(t.shape)}")
-        return t.data_ptr()
+        if t.dtype is not dtype:
+            raise InvalidArgument(120, f"{name} must be {str(dtype)[6:]}, not {str(t.dtype)[6:]}")
+        raise InvalidArgument(120, f"{name} must be {list(shape)}, contiguous; got {list(t.shape)}")
 
-    def _table(self, table, batch: int = -1) -> tuple:
-        torch = _torch()
-        at = self._arg(table, "table", (torch.int32,), (batch, -1))
-        if table.numel() == 0:
-            raise InvalidArgument(120, "an empty page table")
-        return at, table.shape[1], table.shape[0]
+    def _table(self, table) -> tuple:
+        if table.dim() != 2 or table.numel() == 0:
+            raise InvalidArgument(120, "a page table is int32 [batch, width], not empty")
+        batch, width = table.shape
+        return self._arg(table, "table", _torch().int32, (batch, width)), width, batch
 
     def _on(self, stream):
         """A context in which new tensors belong to the stream of the call, and the stream."""
         torch = _torch()
         if stream is None:
-            if torch.cuda.current_device() == self.device.index:
-                return _HERE, torch.cuda.current_stream(self.device).cuda_stream
-            return torch.cuda.device(self.device), torch.cuda.current_stream(self.device).cuda_stream
+            s = torch._C._cuda_getCurrentRawStream(self._index)
+            return (_HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)), s
         if stream.device != self.device:
             raise InvalidArgument(120, f"the stream must be on the pool's device, {self.device}")
         return torch.cuda.stream(stream), stream.cuda_stream
@@ -791,8 +790,8 @@ class KVPages:
         onwards; without offsets row i is sequence i's next token."""
         torch = _torch()
         tp, width, batch = self._table(table)
-        sp = self._arg(starts, "starts", (torch.int32,), (batch,))
-        op = 0 if offsets is None else self._arg(offsets, "offsets", (torch.int32,), (batch + 1,))
+        sp = self._arg(starts, "starts", torch.int32, (batch,))
+        op = 0 if offsets is None else self._arg(offsets, "offsets", torch.int32, (batch + 1,))
         if rows.device != self.device or rows.dtype not in (torch.float16, torch.int16) or \
                 rows.dim() != 4 or tuple(rows.shape[1:]) != (2, self.kv_heads, 128) or rows.stride(3) != 1:
             raise InvalidArgument(120, f"rows must be float16 [n, 2, {self.kv_heads}, 128] on {self.device}")
@@ -806,8 +805,9 @@ class KVPages:
         s2 = rows.stride(2) if self.kv_heads > 1 else 0
         context, s = self._on(stream)
         with context:
-            _raise(lib().hsb_kv_append(self._ref, tp, width, batch, sp, op, k, k + 2 * rows.stride(1), n, s0, s2,
-                                       self._st, s))
+            status = self._lib.hsb_kv_append(self._ref, tp, width, batch, sp, op, k, k + 2 * rows.stride(1), n,
+                                             s0, s2, self._st, s)
+        _raise(status)
 
     def read(self, positions, table, seqs=None, count=None, out=None, stream=None):
         """F16 rows [n, 2, kv_heads, 128] of positions (int32 [n]) of sequences
@@ -815,17 +815,17 @@ class KVPages:
         device): only the first count rows are written."""
         torch = _torch()
         tp, width, batch = self._table(table)
-        pp = self._arg(positions, "positions", (torch.int32, torch.uint32), (-1,))
-        n = positions.shape[0]
-        qp = 0 if seqs is None else self._arg(seqs, "seqs", (torch.int32,), (n,))
-        cp = 0 if count is None else self._arg(count, "count", (torch.int32, torch.uint32), (1,))
+        n = positions.numel()
+        pp = self._arg(positions, "positions", torch.int32, (n,))
+        qp = 0 if seqs is None else self._arg(seqs, "seqs", torch.int32, (n,))
+        cp = 0 if count is None else self._arg(count, "count", torch.int32, (1,))
         context, s = self._on(stream)
         with context:
             if out is None:
                 out = torch.empty((n, 2, self.kv_heads, 128), dtype=torch.float16, device=self.device)
-            dst = self._arg(out, "out", (torch.float16, torch.int16), (n, 2, self.kv_heads, 128))
-            if n:
-                _raise(lib().hsb_kv_read(self._ref, tp, width, batch, qp, pp, cp, n, dst, self._st, s))
+            dst = self._arg(out, "out", torch.float16, (n, 2, self.kv_heads, 128))
+            status = self._lib.hsb_kv_read(self._ref, tp, width, batch, qp, pp, cp, n, dst, self._st, s) if n else 0
+        _raise(status)
         return out
 
     def attention(self, q, table, lengths, out=None, stream=None):
@@ -834,16 +834,18 @@ class KVPages:
         torch = _torch()
         tp, width, batch = self._table(table)
         shape = (batch, 4 * self.kv_heads, 128)
-        qp = self._arg(q, "q", (torch.float32,), shape)
-        np_ = self._arg(lengths, "lengths", (torch.int32,), (batch,))
+        qp = self._arg(q, "q", torch.float32, shape)
+        np_ = self._arg(lengths, "lengths", torch.int32, (batch,))
         context, s = self._on(stream)
         with context:
             if out is None:
                 out = torch.empty(shape, dtype=torch.float32, device=self.device)
-            dst = self._arg(out, "out", (torch.float32,), shape)
-            size = lib().hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
+            dst = self._arg(out, "out", torch.float32, shape)
+            size = self._lib.hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
             ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _raise(lib().hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size, self._st, s))
+            status = self._lib.hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size,
+                                                self._st, s)
+        _raise(status)
         return out
 
     def attention_shared(self, q, table, lengths, prefix: "KVPages", prefix_table, prefix_tokens: int, out=None,
@@ -854,23 +856,24 @@ class KVPages:
         torch = _torch()
         tp, width, batch = self._table(table)
         shape = (batch, 4 * self.kv_heads, 128)
-        qp = self._arg(q, "q", (torch.float16,), shape)
-        np_ = self._arg(lengths, "lengths", (torch.int32,), (batch,))
-        ptp = prefix._arg(prefix_table, "prefix_table", (torch.int32,), (-1,))
+        qp = self._arg(q, "q", torch.float16, shape)
+        np_ = self._arg(lengths, "lengths", torch.int32, (batch,))
+        ptp = self._arg(prefix_table, "prefix_table", torch.int32, (prefix_table.numel(),))
         prefix_tokens = int(prefix_tokens)
         if prefix.device != self.device:
             raise InvalidArgument(120, "the prefix must be on the pool's device")
-        if prefix_tokens < 1 or prefix_tokens > 64 * prefix_table.shape[0]:
+        if prefix_tokens < 1 or prefix_tokens > 64 * prefix_table.numel():
             raise InvalidArgument(120, "prefix_tokens must be 1 .. 64 * len(prefix_table)")
         context, s = self._on(stream)
         with context:
             if out is None:
                 out = torch.empty(shape, dtype=torch.float16, device=self.device)
-            dst = self._arg(out, "out", (torch.float16,), shape)
-            size = lib().hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
+            dst = self._arg(out, "out", torch.float16, shape)
+            size = self._lib.hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
             ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _raise(lib().hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_, batch, qp,
-                                                 dst, ws.data_ptr(), size, self._st, s))
+            status = self._lib.hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_,
+                                                       batch, qp, dst, ws.data_ptr(), size, self._st, s)
+        _raise(status)
         return out
 
 

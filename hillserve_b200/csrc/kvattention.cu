@@ -150,75 +150,61 @@ struct Walker {
     }
 };
 
-// Finds this warp's part of CTA blockIdx.x's stretch.  Every thread of the block calls it.
+// Finds this warp's part of CTA blockIdx.x's stretch.  Each warp scans the
+// lengths by itself (a lane has every 1/32 of the batch): no barrier is needed.
 template <typename R>
 __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, uint32_t* stretch) {
-    constexpr int kThreads = R::kThreads, kWarps = R::kWarps;
-    __shared__ uint32_t warp_sum_s[kWarps], found[kWarps][3];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t batch = (uint32_t)p.batch, per = (batch + kThreads - 1) / kThreads;
-    const uint32_t b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool scribe = blockIdx.x == 0 && warp == 0;
+    const uint32_t batch = (uint32_t)p.batch, per = (batch + 31) / 32;
+    const uint32_t b0 = min(batch, lane * per), b1 = min(batch, b0 + per);
     uint32_t mine = 0;
-    for (uint32_t b = b0; b < b1; ++b) mine += R::units(tokens_of(p, b, blockIdx.x == 0));
+#pragma unroll 8
+    for (uint32_t b = b0; b < b1; ++b) mine += R::units(tokens_of(p, b, scribe));
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
-    if (lane == 31) warp_sum_s[warp] = upto;
-    __syncthreads();
-    uint32_t total = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before = total;
-        total += warp_sum_s[w];
-    }
-    before += upto - mine;  // units (of one head) of the sequences before b0
-    if (p.cum && blockIdx.x == 0) {
+    const uint32_t total = __shfl_sync(0xffffffffu, upto, 31), before = upto - mine;  // units of one head
+    if (p.cum && scribe) {
         uint32_t c = before;
         for (uint32_t b = b0; b < b1; ++b) {
             p.cum[b] = c;
             c += R::units(tokens_of(p, b, false));
         }
-        if (tid == 0) p.cum[batch] = total;
+        if (lane == 0) p.cum[batch] = total;
     }
     const Split ctas(total * p.v.heads, gridDim.x);
     const uint32_t u0 = ctas.begin(blockIdx.x), u1 = ctas.begin(blockIdx.x + 1);
-    const Split parts(u1 - u0, kWarps);
+    const Split parts(u1 - u0, R::kWarps);
     *total_units = total * p.v.heads;
     stretch[0] = u0;
     stretch[1] = u1;
-    // (heads is a power of two)
-    const int shift = 31 - __clz(p.v.heads);
-    if (mine)
-        for (int w = 0; w < kWarps; ++w) {
-            const uint32_t a = u0 + parts.begin(w), rank = a >> shift;
-            if (a == u0 + parts.begin(w + 1) || rank < before || rank >= before + mine) continue;
-            uint32_t b = b0, c = before, n, k;
-            while (true) {
-                n = tokens_of(p, b, false);
-                k = R::units(n);
-                if (rank < c + k) break;
-                c += k;
-                ++b;
-            }
-            found[w][0] = b;
-            found[w][1] = n;
-            found[w][2] = c;
-        }
-    __syncthreads();
     Walker<R> k{};
     k.u = u0 + parts.begin(warp);
     k.end = u0 + parts.begin(warp + 1);
-    if (!k.done()) {
-        k.seq = found[warp][0];
-        k.tokens = found[warp][1];
-        k.units = R::units(k.tokens);
-        const uint32_t base = found[warp][2] << shift;
-        k.head = (int)((k.u - base) / k.units);
-        k.run = base + k.head * k.units;
+    if (k.done()) return k;
+    const int shift = 31 - __clz(p.v.heads);  // heads is a power of two
+    const uint32_t rank = k.u >> shift;       // among the units of one head
+    const bool here = rank >= before && rank < upto;
+    uint32_t b = b0, n = 0, c = before;
+    if (here) {
+        while (true) {
+            n = tokens_of(p, b, false);
+            if (rank < c + R::units(n)) break;
+            c += R::units(n);
+            ++b;
+        }
     }
+    const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    k.seq = __shfl_sync(0xffffffffu, b, src);
+    k.tokens = __shfl_sync(0xffffffffu, n, src);
+    k.units = R::units(k.tokens);
+    const uint32_t base = __shfl_sync(0xffffffffu, c, src) << shift;
+    k.head = (int)((k.u - base) / k.units);
+    k.run = base + k.head * k.units;
     return k;
 }
 
@@ -251,7 +237,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     pdl_wait();
     pdl_trigger();
     uint32_t units, stretch[2];
-    Walker<R> k = find_part<R>(p, &units, stretch);  // syncs: the barriers are ready
+    Walker<R> k = find_part<R>(p, &units, stretch);
+    __syncwarp();  // the barriers are ready
     if (kFinal) {  // empty sequences: zeros
         for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
             if (tokens_of(p, b, false) == 0)
@@ -264,6 +251,17 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         p.info[blockIdx.x] = info;
     }
     if (stretch[0] >= stretch[1]) return;
+
+    const int g = lane >> 2, t = lane & 3;
+    // this lane's share of a run's query head g & 3: for step ks the channels of its K words
+    float4 x4[8];
+    const auto load_query = [&]() {
+        const Q* q = static_cast<const Q*>(p.q) + ((size_t)(k.seq * p.v.heads + k.head) * kGroup + (g & 3)) * kDim;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+            x4[ks] = load_q4(q + (Fmt::kScaled ? t * 32 + ks * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4));
+    };
+    if (!k.done()) load_query();  // on its way while the ring is fed
 
     // ---- feeding: K (even) or V (odd) of unit feed.u into slot fed % kSlots
     Walker<R> feed = k;
@@ -307,7 +305,6 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     for (int i = 0; i < kSlots; ++i)
         if (!feed.done()) feed_one();
 
-    const int g = lane >> 2, t = lane & 3;
     const bool low = t >= 2;     // this lane's accumulator columns are the remainders' (and g >= 4 in B fragments)
     const int h0 = 2 * (t & 1);  // they are heads h0 and h0 + 1 of the group
     // Of a unit's 8-token rows i (tokens 8 i + g), lanes t < 2 do the softmax of the first
@@ -327,15 +324,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         uint32_t bq[8][2];
         float sw[2];
         {
-            const Q* q = static_cast<const Q*>(p.q) + ((size_t)run * kGroup + (g & 3)) * kDim;
-            float4 x[8];
             float top = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-                x[ks] = load_q4(q + (Fmt::kScaled ? t * 32 + ks * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4));
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[ks].x), fabsf(x[ks].y)), fmaxf(fabsf(x[ks].z), fabsf(x[ks].w))));
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x4[ks].x), fabsf(x4[ks].y)), fmaxf(fabsf(x4[ks].z), fabsf(x4[ks].w))));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // per head, 2^e brings max |q| into [2^14, 2^15): neither half leaves F16's normal range
@@ -344,8 +336,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                bq[ks][0] = split_pair(x[ks].x * up, x[ks].y * up, g >= 4);
-                bq[ks][1] = split_pair(x[ks].z * up, x[ks].w * up, g >= 4);
+                bq[ks][0] = split_pair(x4[ks].x * up, x4[ks].y * up, g >= 4);
+                bq[ks][1] = split_pair(x4[ks].z * up, x4[ks].w * up, g >= 4);
             }
             const float s = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
             sw[0] = __shfl_sync(0xffffffffu, s, h0 * 4);
@@ -538,6 +530,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             ++it;
         }
         if (!alive) break;
+        const bool begins = run_begin >= begin, ends = run_end <= k.end, whole = begins && ends;
+        k.u = stop - 1;  // to the next run
+        k.step(p);
+        if (!k.done()) load_query();
         // ---------------- the run's end here: all rows' sums, rounding + remainder
         const float os = Fmt::kScaled ? vref / kWeightUnit : 1.0f / kWeightUnit;
 #pragma unroll
@@ -551,7 +547,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[j][r] = (o[j][r] + __shfl_xor_sync(0xffffffffu, o[j][r], 2)) * os;
-        const bool begins = run_begin >= begin, ends = run_end <= k.end, whole = begins && ends;
+        // a whole run's results, or a piece in shared memory: one that goes on is the part's
+        // last, so the ring has no more copies in flight and keeps it
         if (!whole && lane == 0) {
             Piece& c = pieces[warp][begins];
             c.id = run;
@@ -580,8 +577,6 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
                 }
             }
         }
-        k.u = stop - 1;  // to the next run
-        k.step(p);
     }
     if (!alive) {  // gave up: copies in flight land before shared memory is released
         if (lane == 0) raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
@@ -597,15 +592,19 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         const bool begins = c.first >= stretch[0], ends = c.last <= stretch[1];
         for (int i = tid; i < kGroup * kDim / 2; i += kThreads) {
             const int h = i >> 6, at = 2 * kGroup + i * 2;
-            float top = -INFINITY;
-            for (int w = w0; w <= w1; ++w)
-                if (w == w0 || pieces[w][0].there) top = fmaxf(top, piece_at(w, w == w0 && which)[2 * h]);
-            float sum = 0.0f, a = 0.0f, b = 0.0f;
-            for (int w = w0; w <= w1; ++w) {
-                if (w != w0 && !pieces[w][0].there) continue;
+            float m[kWarps], top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const bool member = w == w0 || (w > w0 && w <= w1 && pieces[w][0].there);
+                m[w] = member ? piece_at(w, w == w0 && which)[2 * h] : INFINITY;
+                if (member) top = fmaxf(top, m[w]);
+            }
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (m[w] == INFINITY) continue;
                 const float* part = piece_at(w, w == w0 && which);
                 // (no token under a finite maximum: sum 0; a NaN sum comes through)
-                const float f = top == -INFINITY ? 1.0f : exp2f(part[2 * h] - top);
+                const float f = top == -INFINITY ? 1.0f : exp2_ftz(m[w] - top);
                 const float2 v = *reinterpret_cast<const float2*>(part + at);
                 sum = fmaf(f, part[2 * h + 1], sum);
                 a = fmaf(f, v.x, a);
@@ -654,50 +653,49 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
 
 // Folds the partials of the run that begins in CTA blockIdx.x's stretch and
 // does not end there, in the order of the CTAs (a run that goes on leaves no
-// empty stretch before its end).  Thread = (head, channel).
-__global__ void __launch_bounds__(kGroup* kDim) kv_combine_kernel(const float* __restrict__ part,
-                                                                 const RunInfo* __restrict__ infos,
-                                                                 float* __restrict__ out) {
-    __shared__ float weight[kGroup][kAttnMaxCtas];
-    __shared__ float inv[kGroup];
+// empty stretch before its end): head blockIdx.y, thread = channel.  Every load
+// of the first 32 partials' weights and 8 outputs is on its way before the
+// run's extent is known; what lies behind it is not used.
+__global__ void __launch_bounds__(kDim) kv_combine_kernel(const float* __restrict__ part, const RunInfo* __restrict__ infos,
+                                                         float* __restrict__ out) {
+    constexpr int kFirst = 8;
     pdl_wait();
     pdl_trigger();
-    const RunInfo info = infos[blockIdx.x];
-    if (info.run < 0) return;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n = (int)(info.last - blockIdx.x) + 1;
+    const int h = blockIdx.y, d = threadIdx.x, lane = d & 31;
+    const int room = (int)(gridDim.x - blockIdx.x);  // partials that there can be
     // the first partial is its CTA's [1], the others their CTAs' [0]
     const float* base = part + (size_t)blockIdx.x * 2 * kPartFloats;
     const auto at = [&](int i) { return base + ((size_t)i * 2 + (i == 0)) * kPartFloats; };
-    if (warp < kGroup) {  // weights of the partials of head `warp`
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) {
-            const float m = __ldcg(at(i) + 2 * warp);
-            weight[warp][i] = m;
-            top = fmaxf(top, m);
-        }
-        top = warp_max(top);
-        float sum = 0.0f;
-        for (int i = lane; i < n; i += 32) {
-            const float f = top == -INFINITY ? 1.0f : exp2f(weight[warp][i] - top);
-            weight[warp][i] = f;
-            sum = fmaf(f, __ldcg(at(i) + 2 * warp + 1), sum);
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) inv[warp] = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
-    }
-    float first[8];  // the first outputs are on their way meanwhile
+    const RunInfo info = infos[blockIdx.x];
+    float2 ml = lane < room ? __ldcg(reinterpret_cast<const float2*>(at(lane) + 2 * h)) : make_float2(0.0f, 0.0f);
+    float v[kFirst];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) first[i] = i < n ? __ldcg(at(i) + 2 * kGroup + tid) : 0.0f;
-    __syncthreads();
-    const int h = tid / kDim;
-    float acc = 0.0f;
+    for (int i = 0; i < kFirst; ++i) v[i] = i < room ? __ldcg(at(i) + 2 * kGroup + h * kDim + d) : 0.0f;
+    if (info.run < 0) return;
+    const int n = (int)(info.last - blockIdx.x) + 1;
+    float M = -INFINITY, L = 0.0f, acc = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0) ml = i0 + lane < n ? __ldcg(reinterpret_cast<const float2*>(at(i0 + lane) + 2 * h)) : make_float2(0.0f, 0.0f);
+        const bool some = i0 + lane < n;
+        const float top = fmaxf(M, warp_max(some ? ml.x : -INFINITY));
+        // (all -infinity: no token, sum 0; a NaN sum comes through)
+        const float old = M == -INFINITY ? 0.0f : exp2_ftz(M - top);
+        const float f = !some ? 0.0f : top == -INFINITY ? 1.0f : exp2_ftz(ml.x - top);
+        L = L * old + warp_sum(some ? f * ml.y : 0.0f);
+        acc *= old;
+        M = top;
+        const int m = min(32, n - i0);
+        int i = 0;
+        if (i0 == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) acc = fmaf(weight[h][i], first[i], acc);
+            for (i = 0; i < kFirst; ++i)
+                if (i < m) acc = fmaf(__shfl_sync(0xffffffffu, f, i), v[i], acc);
+        }
 #pragma unroll 8
-    for (int i = 8; i < n; ++i) acc = fmaf(weight[h][i], __ldcg(at(i) + 2 * kGroup + tid), acc);
-    out[(size_t)info.run * kGroup * kDim + tid] = acc * inv[h];
+        for (; i < m; ++i)
+            acc = fmaf(__shfl_sync(0xffffffffu, f, i), __ldcg(at(i0 + i) + 2 * kGroup + h * kDim + d), acc);
+    }
+    out[((size_t)info.run * kGroup + h) * kDim + d] = acc * (L > 0.0f ? 1.0f / L : (L == L ? 0.0f : L));
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -771,7 +769,7 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     const unsigned grid = paged_attention_grid(batch * table_width * pages->kv_heads);
     cudaError_t e = launch_format<float, true>(pages->format, p, grid, s);
     if (e == cudaSuccess)
-        e = launch_dependent(kv_combine_kernel, dim3(grid), dim3(kGroup * kDim), 0, s, false,
+        e = launch_dependent(kv_combine_kernel, dim3(grid, kGroup), dim3(kDim), 0, s, false,
                              static_cast<const float*>(p.part), static_cast<const RunInfo*>(p.info), p.out);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
     record_error(HSB_OK, "");
