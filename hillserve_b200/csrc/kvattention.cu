@@ -52,6 +52,8 @@ constexpr float kSlack = 8.0f;
 // Each warp's ring holds K and V of its units in turn (K 0, V 0, K 1, ...): a
 // slot is free again as soon as its product is done.  A unit is a page in 8
 // bits; in F16, twice the bytes a token and no codes to convert, half a page.
+// The scales of both come with V (they follow it in the page: one copy), as
+// the logits are first needed where the weights are made.
 template <int F>
 struct Ring {
     using Fmt = PageFormat<F>;
@@ -61,8 +63,8 @@ struct Ring {
     static constexpr int kTokens = F == HSB_KV_F16 ? kPageTokens / 2 : kPageTokens;  // of a unit
     static constexpr int kPerPage = kPageTokens / kTokens;
     static constexpr int kPanel = kTokens * 128;
-    static constexpr int kScales = Fmt::kPanels * kPanel;
-    static constexpr int kSlot = kScales + (Fmt::kScaled ? kTokens * 4 : 0);
+    static constexpr int kPart = Fmt::kPanels * kPanel;  // K or V of a unit; the scales lie behind V
+    static constexpr int kSlot = kPart + (Fmt::kScaled ? 2 * kTokens * 4 : 0);
     static constexpr int kSmem = 128 + kWarps * (kSlots * kSlot + kPartFloats * 4);
     static_assert(kSlots * kSlot >= kPartFloats * 4, "a piece fits in a warp's ring");
     __host__ __device__ static constexpr uint32_t units(uint32_t tokens) { return (tokens + kTokens - 1) / kTokens; }
@@ -108,6 +110,12 @@ __device__ __forceinline__ float4 load_q4(const uint16_t* q) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 // 2^x; a result below the normal range is 0.
 __device__ __forceinline__ float exp2_ftz(float x) {
     float y;
@@ -159,7 +167,7 @@ __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, u
     const uint32_t batch = (uint32_t)p.batch, per = (batch + 31) / 32;
     const uint32_t b0 = min(batch, lane * per), b1 = min(batch, b0 + per);
     uint32_t mine = 0;
-#pragma unroll 8
+#pragma unroll 4
     for (uint32_t b = b0; b < b1; ++b) mine += R::units(tokens_of(p, b, scribe));
     uint32_t upto = mine;
 #pragma unroll
@@ -279,19 +287,23 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             }
             id = __shfl_sync(0xffffffffu, ids, (int)(page - ids_first));
         }
-        if (lane == 0) {
+        if (elect_one()) {
             if (id >= 0 && (unsigned long long)id < p.v.pages) {
                 const int half = (int)((feed.u - feed.run) % R::kPerPage);
                 const unsigned char* src = p.v.data + ((size_t)id * p.v.heads + feed.head) * Fmt::kBytes;
                 unsigned char* dst = ring + s * R::kSlot;
                 bad[s] = 0;
-                mbar_arrive_expect_tx(&full[s], R::kSlot);
+                if constexpr (Fmt::kScaled) {
+                    const uint32_t bytes = part ? R::kSlot : R::kPart;
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                    bulk_copy_g2s(dst, src + part * R::kPart, bytes, &full[s]);
+                } else {
+                    mbar_arrive_expect_tx(&full[s], R::kPart);
 #pragma unroll
-                for (int i = 0; i < Fmt::kPanels; ++i)
-                    bulk_copy_g2s(dst + i * R::kPanel, src + (part * Fmt::kPanels + i) * kPanelBytes + half * R::kPanel,
-                                  R::kPanel, &full[s]);
-                if constexpr (Fmt::kScaled)
-                    bulk_copy_g2s(dst + R::kScales, src + Fmt::kScaleOffset + part * kPageTokens * 4, kPageTokens * 4, &full[s]);
+                    for (int i = 0; i < Fmt::kPanels; ++i)
+                        bulk_copy_g2s(dst + i * R::kPanel, src + (part * Fmt::kPanels + i) * kPanelBytes + half * R::kPanel,
+                                      R::kPanel, &full[s]);
+                }
             } else {  // no such page: its tokens are left out
                 if (part == 0) raise_status(p.status, HSB_E_KV_PAGE, (int)feed.seq);
                 bad[s] = 1;
@@ -301,7 +313,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         if (part) fresh = feed.step(p);
         ++fed;
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kSlots; ++i)
         if (!feed.done()) feed_one();
 
@@ -391,20 +403,6 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
                         x[j][e] = (low ? b : a) + __shfl_xor_sync(0xffffffffu, low ? a : b, 2);
                     }
             }
-            if constexpr (Fmt::kScaled) {
-#pragma unroll
-                for (int e = 0; e < kTiles; ++e) {
-                    const float ks = lds32(blk + R::kScales + (token0 + 8 * e) * 4);
-                    x[0][e] *= sw[0] * ks;
-                    x[1][e] *= sw[1] * ks;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < kTiles; ++e) {
-                    x[0][e] *= sw[0];
-                    x[1][e] *= sw[1];
-                }
-            }
             __syncwarp();  // the slot is read
             if (!feed.done()) feed_one();
             ++it;
@@ -415,9 +413,15 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             if (!skip) {
                 blk = smem_addr(ring + s * R::kSlot);
                 float vs[kTiles];
-                if constexpr (Fmt::kScaled) {
 #pragma unroll
-                    for (int e = 0; e < kTiles; ++e) vs[e] = lds32(blk + R::kScales + (token0 + 8 * e) * 4);
+                for (int e = 0; e < kTiles; ++e) {
+                    float ks = 1.0f;
+                    if constexpr (Fmt::kScaled) {
+                        ks = lds32(blk + R::kPart + (token0 + 8 * e) * 4);
+                        vs[e] = lds32(blk + R::kPart + (kPageTokens + token0 + 8 * e) * 4);
+                    }
+                    x[0][e] *= sw[0] * ks;
+                    x[1][e] *= sw[1] * ks;
                 }
                 if (live < R::kTokens) {
 #pragma unroll
@@ -631,24 +635,21 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         }
     };
     int open = -1, which = 0, last = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (pieces[w][0].there) {
-            if (open < 0) {
+    for (int i = 0; i <= 2 * kWarps; ++i) {  // the pieces in order: a run's are neighbours
+        const int w = i >> 1, second = i & 1;
+        const bool there = i < 2 * kWarps && pieces[w][second].there;
+        if (there) {
+            if (second || open < 0) {
                 open = w;
-                which = 0;
+                which = second;
             }
             last = w;
-            if (pieces[w][0].ends) {
-                fold_run(open, which, w);
-                open = -1;
-            }
         }
-        if (pieces[w][1].there) {
-            open = last = w;
-            which = 1;
+        if (open >= 0 && (i == 2 * kWarps || (there && !second && pieces[w][0].ends))) {
+            fold_run(open, which, last);
+            open = -1;
         }
     }
-    if (open >= 0) fold_run(open, which, last);
 }
 
 // Folds the partials of the run that begins in CTA blockIdx.x's stretch and
