@@ -116,16 +116,8 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
     return one != 0;
 }
-// 2^x; a result below the normal range is 0.
-__device__ __forceinline__ float exp2_ftz(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Tokens of a sequence; a length behind the table's end counts as none.
 __device__ __forceinline__ uint32_t tokens_of(const PagedAttention& p, uint32_t b, bool report) {
-    if (!p.lengths) return p.length;
     const int32_t n = p.lengths[b];
     if (n < 0 || (unsigned long long)n > p.v.width * kPageTokens) {
         if (report) raise_status(p.status, HSB_E_KV_POSITION, (int)b);

@@ -9,6 +9,7 @@ constexpr unsigned kAttnMaxCtas = 512;
 constexpr int kPartFloats = kGroup * 2 + kGroup * kDim;  // (max in log2 units, sum) per head, then the outputs
 constexpr size_t kMaxBatch = 1u << 20;
 constexpr size_t kMaxTableEntries = 1ull << 27;  // keeps the units of 8 heads within 32 bits
+constexpr size_t kMaxPrefix = 1ull << 30;
 // log2(e) / sqrt(128): logits in the unit of exp2
 constexpr float kScaleLog2 = 1.4426950408889634f * 0.08838834764831845f;
 
@@ -20,8 +21,7 @@ struct RunInfo {
 
 struct PagedAttention {
     PagedView v;
-    const int32_t* lengths;      // [batch], or null: `length` for every sequence
-    unsigned long long length;
+    const int32_t* lengths;      // [batch]
     unsigned long long batch;
     const void* q;               // [batch][4 heads][128]
     float* out;                  // final mode: F32 [batch][4 heads][128]
@@ -44,6 +44,13 @@ struct Split {
         return u < longer ? u / (each + 1) : more + (u - longer) / each;
     }
 };
+
+// 2^x; a result below the normal range is 0.
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 unsigned paged_attention_grid(size_t units);
 cudaError_t launch_paged_partials(int format, const PagedAttention& p, unsigned grid, cudaStream_t stream);

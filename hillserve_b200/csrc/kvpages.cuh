@@ -36,7 +36,7 @@ struct PagedView {
     int heads;
     const int32_t* table;           // [batch][pitch]
     unsigned long long width;       // entries of a sequence
-    unsigned long long pitch;       // 0: every sequence has the first's
+    unsigned long long pitch;       // entries from one sequence to the next
 };
 
 // The pool page of a sequence's position, -1 (with a status) where the table

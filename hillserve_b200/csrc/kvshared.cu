@@ -1,4 +1,26 @@
 // kvshared.cu -- decode attention of a batch whose sequences share a prefix.
+//
+// The prefix is where the arithmetic is: every row of the batch (four query
+// heads to a sequence and KV head) meets the same K and V, so the batch's rows
+// are the M dimension of two real matrix products and the prefix is read once
+// (for 64 sequences; again from L2 for each further 64).  kv_prefix_kernel runs
+// them on the tensor cores' own pipeline:
+//
+//   S[row][token] = Q K^T      A = Q (shared memory), B = K (shared memory, K-major)
+//   O[row][ch]   += P V        A = P (tensor memory), B = V (shared memory, MN-major)
+//
+// with M = 128 rows (32 sequences), tiles of 128 tokens, both accumulators in
+// tensor memory.  A page's F16 panels already are the operands' 128-byte
+// swizzled layout, so the loader is four 8 KB bulk copies a tile and operand.
+// Two warpgroups own one M tile each: thread = row reads its 128 logits from
+// tensor memory, forms the weights without any exchange and writes them back
+// as F16 over the logits; while one softmax runs, the other tile's products do.
+// For at most 32 sequences there is one M tile, and the two warpgroups take the
+// even and the odd tokens' tiles of it instead.
+//
+// The (KV head, M tiles, token tile) units are split evenly over the SMs; each
+// stretch of a run leaves F32 partials.  The sequences' own tokens go through
+// the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
 #include <algorithm>
 
 #include "kvattention.cuh"
@@ -6,66 +28,553 @@
 namespace hsb {
 namespace {
 
-// Partial results of one run: `n` of them, from the stretches first, first + 1, ...
-struct Source {
-    const float* part;
-    const float* whole;
-    uint32_t units;
-    unsigned ctas;
+constexpr int kTileRows = 128, kTileTokens = 128;
+constexpr int kTileSeqs = kTileRows / kGroup;
+constexpr int kTileBytes = kTileTokens * 256;       // K or V of a tile; also a Q tile
+constexpr int kTilePanel = kTileTokens * 128;       // its 64-channel half
+constexpr int kSoftmaxThreads = 256;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kPrefixThreads = 320;
+constexpr unsigned kPrefixMaxCtas = 160;
+constexpr float kSlack = 8.0f;                      // weights are at most 2^8 (F16 holds 2^15)
+constexpr int kLive = 16;                           // ring of tiles' live counts
+// a partial: outputs [32 channel quads][128 rows][4], then (max, sum) [128 rows]
+constexpr int kRowsFloats = kTileRows * kDim + 2 * kTileRows;
+
+// kDual: one M tile, the warpgroups take alternate token tiles.
+template <bool kDual>
+struct Plan {
+    static constexpr int kQBytes = (kDual ? 1 : 2) * kTileBytes;
+    static constexpr int kStages = kDual ? 6 : 5;
+    static constexpr int kSmem = 1024 + kQBytes + kStages * kTileBytes;
 };
 
+struct PrefixParams {
+    PagedView v;         // the prefix pool; table [ceil(tokens / 64)]
+    uint32_t tokens, tiles;
+    const uint16_t* q;   // F16 [batch][4 heads][128]
+    uint32_t batch, groups;  // groups: of M tiles (one or two)
+    uint32_t runs;       // heads x groups
+    float* part;         // [stretch + run][2][kRowsFloats]
+    hsb_device_status* status;
+    float scale_log2;
+};
+
+// ---------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t* out, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(out)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives on `bar` when every product this thread issued has completed.
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+// Descriptor of a 128-byte-swizzled operand: 8-row groups 1024 bytes apart, and
+// for an MN-major one the 64-element halves `leading` bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// F16 operands, F32 accumulator, M = N = 128; B K-major or MN-major.
+constexpr uint32_t kShapeK = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kShapeMN = kShapeK | (1u << 16);
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+// 32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_load32(uint32_t at, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Generic writes to shared memory before the tensor cores or bulk copies use it.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Waits for a phase; gives up after kWaitLimitNs or once another role did.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long start = global_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (*dead || global_ns() - start > kWaitLimitNs) {
+            *dead = 1;
+            return false;
+        }
+    return true;
+}
+
+// A CTA's stretch of units, one segment (the part of a run) at a time.
+struct Segment {
+    uint32_t u, end, tiles;
+    __device__ bool done() const { return u >= end; }
+    __device__ uint32_t run() const { return u / tiles; }
+    __device__ uint32_t first() const { return u % tiles; }
+    __device__ uint32_t count() const { return min(end - u, tiles - first()); }
+    __device__ void next() { u += count(); }
+};
+
+template <bool kDual>
+__global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __grid_constant__ PrefixParams p) {
+    using P = Plan<kDual>;
+    constexpr int kStages = P::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2];
+    __shared__ uint32_t tmem_s;
+    __shared__ int live_s[kLive][2];  // tokens of a tile's two pages that count
+    __shared__ volatile int dead;
+    unsigned char* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    const uint32_t q_s = smem_addr(smem), ring_s = q_s + P::kQBytes;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&q_full, kSoftmaxThreads);
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(&s_full[w], 1);
+            mbar_init(&p_full[w], 128);
+            mbar_init(&o_full[w], 1);
+        }
+        mbar_fence_init();
+        dead = 0;
+    }
+    if (warp == kMmaWarp) tmem_alloc(&tmem_s, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;  // columns: S 0, S 1, O 0, O 1 (128 each); P over the front of S
+    pdl_wait();
+    pdl_trigger();
+    const Split split(p.runs * p.tiles, gridDim.x);
+    Segment seg{split.begin(blockIdx.x), split.begin(blockIdx.x + 1), p.tiles};
+
+    if (warp == kLoadWarp) {
+        // ================ loader: K and V tiles in the order the products take them
+        uint32_t it = 0;
+        bool ok = true;
+        const auto load = [&](uint32_t tile, int head, int part, uint32_t number) {
+            const uint32_t s = it % kStages;
+            if (it >= (uint32_t)kStages) ok = ok && __all_sync(0xffffffffu, wait_phase(&empty[s], ((it / kStages) - 1) & 1, &dead));
+            if (!ok) return;
+            const uint32_t token = tile * kTileTokens + (lane & 1) * kPageTokens;
+            int32_t id = -1;
+            int live = 0;
+            if (lane < 2 && token < p.tokens) {
+                id = p.v.table[token / kPageTokens];
+                if (id < 0 || (unsigned long long)id >= p.v.pages) {
+                    id = -1;  // no such page: its tokens are left out
+                    if (part == 0) raise_status(p.status, HSB_E_KV_PAGE, 0);
+                } else {
+                    live = (int)min(p.tokens - token, (uint32_t)kPageTokens);
+                }
+            }
+            if (lane < 2 && part == 0) live_s[number % kLive][lane] = live;
+            const unsigned have = __ballot_sync(0xffffffffu, id >= 0);
+            __syncwarp();
+            if (lane == 0) {
+                if (have) mbar_arrive_expect_tx(&full[s], __popc(have) * 2 * kPanelBytes);
+                else mbar_arrive(&full[s]);
+            }
+            __syncwarp();
+            if (id >= 0) {
+                const unsigned char* src = p.v.data + ((size_t)id * p.v.heads + head) * PageFormat<HSB_KV_F16>::kBytes;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    bulk_copy_g2s(smem + P::kQBytes + s * kTileBytes + i * kTilePanel + lane * kPanelBytes,
+                                  src + (part * 2 + i) * kPanelBytes, kPanelBytes, &full[s]);
+            }
+            __syncwarp();
+            ++it;
+        };
+        uint32_t number = 0;  // tiles of earlier segments
+        for (; ok && !seg.done(); seg.next()) {
+            const int head = (int)(seg.run() / p.groups);
+            const uint32_t first = seg.first(), n = seg.count();
+            load(first, head, 0, number);
+            for (uint32_t i = 0; ok && i < n; ++i) {
+                if (kDual && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
+                if (ok) load(first + i, head, 1, number + i);
+                if (!kDual && ok && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
+            }
+            number += n;
+        }
+        if (!ok) {  // copies in flight land before shared memory is released
+            const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0;
+            for (uint32_t j = from; j < it; ++j) (void)mbar_wait(&full[j % kStages], (j / kStages) & 1);
+        }
+    } else if (warp == kMmaWarp) {
+        // ================ products
+        uint32_t it = 0, number = 0, segment = 0, weights[2] = {0, 0};
+        bool ok = true;
+        const auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+            ok = ok && __all_sync(0xffffffffu, wait_phase(bar, parity, &dead));
+        };
+        const auto take = [&]() {  // the next stage, filled
+            const uint32_t s = it % kStages;
+            wait_all(&full[s], (it / kStages) & 1);
+            ++it;
+            return s;
+        };
+        const auto logits = [&](int w, uint32_t s) {
+            if (ok && lane == 0) {
+                const uint32_t a = q_s + (kDual ? 0 : w * kTileBytes), b = ring_s + s * kTileBytes;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t at = (k >> 2) * kTilePanel + (k & 3) * 32;
+                    tc_mma(tmem + w * 128, operand(a + at, 16), operand(b + at, 16), kShapeK, k > 0);
+                }
+                tc_commit(&s_full[w]);
+            }
+            __syncwarp();
+        };
+        const auto output = [&](int w, uint32_t s, bool add) {
+            wait_all(&p_full[w], weights[w]++ & 1);
+            tc_fence_after();
+            if (ok && lane == 0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + k * 8,
+                                operand(ring_s + s * kTileBytes + k * 16 * 128, kTilePanel), kShapeMN, add || k > 0);
+            }
+            __syncwarp();
+        };
+        // rows of V behind the last token (or of a page that is not there) may hold NaN: zero them
+        const auto clean = [&](uint32_t s, uint32_t tile_number) {
+            if (!ok) return;
+            const int l0 = live_s[tile_number % kLive][0], l1 = live_s[tile_number % kLive][1];
+            if (l0 == kPageTokens && l1 == kPageTokens) return;
+            for (int i = lane; i < kTileTokens * 16; i += 32) {
+                const int row = i >> 4, c = i & 15;
+                if (row < kPageTokens ? row >= l0 : row - kPageTokens >= l1)
+                    *reinterpret_cast<uint4*>(smem + P::kQBytes + s * kTileBytes + (c >> 3) * kTilePanel + row * 128 +
+                                              (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_shared();
+            __syncwarp();
+        };
+        const auto commit = [&](uint64_t* bar) {
+            if (ok && lane == 0) tc_commit(bar);
+            __syncwarp();
+        };
+        for (; ok && !seg.done(); seg.next(), ++segment) {
+            const uint32_t n = seg.count();
+            wait_all(&q_full, segment & 1);
+            tc_fence_after();
+            if constexpr (kDual) {
+                for (uint32_t i = 0; i < 2 && i < n; ++i) {
+                    const uint32_t s = take();
+                    logits(i, s);
+                    commit(&empty[s]);
+                }
+                for (uint32_t i = 0; ok && i < n; ++i) {
+                    const int w = i & 1;
+                    const uint32_t s = take();
+                    clean(s, number + i);
+                    output(w, s, i >= 2);
+                    commit(&empty[s]);
+                    if (i + 2 < n) {
+                        const uint32_t next = take();
+                        logits(w, next);
+                        commit(&empty[next]);
+                    } else {
+                        commit(&o_full[w]);
+                    }
+                }
+                if (n == 1) commit(&o_full[1]);
+            } else {
+                uint32_t s = take();
+                logits(0, s);
+                logits(1, s);
+                commit(&empty[s]);
+                for (uint32_t i = 0; ok && i < n; ++i) {
+                    const uint32_t v = take();
+                    clean(v, number + i);
+                    output(0, v, i > 0);
+                    if (i + 1 < n) {
+                        s = take();
+                        logits(0, s);
+                    } else {
+                        commit(&o_full[0]);
+                    }
+                    output(1, v, i > 0);
+                    commit(&empty[v]);
+                    if (i + 1 < n) {
+                        logits(1, s);
+                        commit(&empty[s]);
+                    } else {
+                        commit(&o_full[1]);
+                    }
+                }
+            }
+            number += n;
+        }
+    } else {
+        // ================ softmax: warpgroup w, thread = row
+        const int w = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + w * 128, o_at = tmem + lanes + 256 + w * 128;
+        uint32_t logits_seen = 0, number = 0, segment = 0;
+        bool ok = true;
+        for (; ok && !seg.done(); seg.next(), ++segment) {
+            const uint32_t run = seg.run(), n = seg.count();
+            const int head = (int)(run / p.groups);
+            const uint32_t mtile = (run % p.groups) * 2;
+            // ---- Q into its operand layout (the products of the last segment are done: o_full)
+            for (int i = 0; i < (kDual ? 8 : 16); ++i) {
+                const int at = kDual ? i * 256 + tid : i * 128 + row;
+                const int r = at >> 4, c = at & 15;
+                const uint32_t seq = (mtile + (kDual ? 0 : w)) * kTileSeqs + r / kGroup;
+                uint4 x = make_uint4(0, 0, 0, 0);  // rows behind the batch
+                if (seq < p.batch)
+                    x = *reinterpret_cast<const uint4*>(
+                        p.q + (((size_t)seq * p.v.heads + head) * kGroup + r % kGroup) * kDim + c * 8);
+                *reinterpret_cast<uint4*>(smem + (kDual ? 0 : w * kTileBytes) + (c >> 3) * kTilePanel + r * 128 +
+                                          (((c & 7) ^ (r & 7)) << 4)) = x;
+            }
+            fence_async_shared();
+            mbar_arrive(&q_full);
+            float m = -INFINITY, l = 0.0f;  // the reference in log2 units; the sum
+            const uint32_t step = kDual ? 2 : 1, first = kDual ? w : 0;
+            for (uint32_t i = first; ok && i < n; i += step) {
+                ok = __all_sync(0xffffffffu, wait_phase(&s_full[w], logits_seen++ & 1, &dead));
+                if (!ok) break;
+                tc_fence_after();
+                float x[kTileTokens];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, x + c * 32);
+                tmem_wait_load();
+                const int l0 = live_s[(number + i) % kLive][0], l1 = live_s[(number + i) % kLive][1];
+                if (l0 < kPageTokens || l1 < kPageTokens) {
+#pragma unroll
+                    for (int j = 0; j < kTileTokens; ++j)
+                        if (j < kPageTokens ? j >= l0 : j - kPageTokens >= l1) x[j] = -INFINITY;
+                }
+                float top = x[0];
+#pragma unroll
+                for (int j = 1; j < kTileTokens; ++j) top = fmaxf(top, x[j]);
+                top *= p.scale_log2;
+                if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                    const float to = fmaxf(m, top);
+                    const float f = m == -INFINITY ? 0.0f : exp2_ftz(m - to);
+                    l *= f;
+                    m = to;
+                    if (i != first) {  // (the first product overwrites O; later ones are complete: s_full)
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            float o[32];
+                            tmem_load32(o_at + c * 32, o);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] *= f;
+                            tmem_store32(o_at + c * 32, reinterpret_cast<const uint32_t*>(o));
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                uint32_t h[kTileTokens / 2];
+                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < kTileTokens; j += 2) {
+                    const float a = exp2_ftz(fmaf(x[j], p.scale_log2, -base));
+                    const float b = exp2_ftz(fmaf(x[j + 1], p.scale_log2, -base));
+                    sums[(j >> 1) & 3] += a + b;
+                    const __half2 pair = __floats2half2_rn(a, b);
+                    h[j >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
+                }
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                tmem_store32(s_at, h);
+                tmem_store32(s_at + 32, h + 32);
+                tmem_wait_store();
+                tc_fence_before();
+                mbar_arrive(&p_full[w]);
+            }
+            // ---- the segment's partial
+            if (ok) ok = __all_sync(0xffffffffu, wait_phase(&o_full[w], segment & 1, &dead));
+            if (!ok) break;
+            tc_fence_after();
+            float* out = p.part + ((size_t)(blockIdx.x + run) * 2 + w) * kRowsFloats;
+            reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(m, l);
+            if (n > first) {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    tmem_load32(o_at + c * 32, o);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        reinterpret_cast<float4*>(out)[(c * 8 + j) * kTileRows + row] =
+                            make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+            } else {  // no tile for this warpgroup
+                for (int c = 0; c < 32; ++c)
+                    reinterpret_cast<float4*>(out)[c * kTileRows + row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            tc_fence_before();
+            number += n;
+        }
+    }
+    __syncthreads();
+    if (tid == 0 && dead) raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
+    tc_fence_after();
+    if (warp == kMmaWarp) {
+        if (dead) {  // products in flight end before tensor memory is freed
+            if (lane == 0) {
+                mbar_init(&q_full, 1);
+                mbar_fence_init();
+                tc_commit(&q_full);
+                (void)mbar_wait(&q_full, 0);
+            }
+            __syncwarp();
+        }
+        tmem_free(tmem, 512);
+    }
+}
+
+// ---------------------------------------------------------------- combine
 struct SharedCombine {
-    Source prefix, own;
-    uint32_t prefix_units;
+    // the prefix: partials [stretch + run][2][kRowsFloats]
+    const float* prefix;
+    uint32_t tiles, groups, runs;
+    unsigned prefix_ctas;
+    int dual;
+    // the sequences' own tokens (kvattention.cuh)
+    const float* part;
+    const float* whole;
     const uint32_t* cum;
-    unsigned long long batch;
+    unsigned own_ctas;
+    uint32_t batch;
     int heads;
     uint16_t* out;
 };
 
-__device__ __forceinline__ void fold(const Source& s, unsigned long long run, unsigned long long begin,
-                                     unsigned long long pages, int h, int d, float& M, float& L, float& acc) {
-    if (!pages) return;
-    const Split split(s.units, s.ctas);
-    const unsigned first = split.of((uint32_t)begin), last = split.of((uint32_t)(begin + pages - 1));
-    for (unsigned c = first; c <= last; ++c) {
-        const float* slot = first == last ? s.whole + run * kPartFloats
-                                          : s.part + ((size_t)c * 2 + (c == first)) * kPartFloats;
-        const float m = __ldcg(slot + 2 * h), l = __ldcg(slot + 2 * h + 1);
-        const float v = __ldcg(slot + 2 * kGroup + h * kDim + d);
-        if (m == -INFINITY && l == l) continue;
-        const float top = fmaxf(M, m), a = M == -INFINITY ? 0.0f : exp2f(M - top), b = top == -INFINITY ? 1.0f : exp2f(m - top);
+struct Fold {
+    float M = -INFINITY, L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __device__ void add(float m, float l, float4 v) {
+        if (m == -INFINITY && l == l) return;  // no token (a NaN sum comes through)
+        const float top = fmaxf(M, m);
+        const float a = M == -INFINITY ? 0.0f : exp2_ftz(M - top), b = top == -INFINITY ? 1.0f : exp2_ftz(m - top);
         L = L * a + l * b;
-        acc = acc * a + v * b;
+        acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
         M = top;
     }
-}
+};
 
-__global__ void __launch_bounds__(kGroup* kDim) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
+// CTA = (two sequences, KV head): thread = (row of the two sequences' eight, channel quad).
+__global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
     pdl_wait();
     pdl_trigger();
-    const unsigned long long run = blockIdx.x, seq = run / p.heads;
-    const int head = (int)(run % p.heads), h = threadIdx.x / kDim, d = threadIdx.x % kDim;
-    float M = -INFINITY, L = 0.0f, acc = 0.0f;
-    Source p_own = p.own;
-    fold(p.prefix, run, run * p.prefix_units, p.prefix_units, h, d, M, L, acc);
-    const unsigned long long pages = p.cum[seq + 1] - p.cum[seq];
-    p_own.units = p.cum[p.batch] * p.heads;
-    fold(p_own, run, p.cum[seq] * p.heads + head * pages, pages, h, d, M, L, acc);
-    p.out[(run * kGroup + h) * kDim + d] = __half_as_ushort(__float2half_rn(L > 0.0f ? acc / L : (L == L ? 0.0f : L)));
+    const int head = blockIdx.y, r8 = threadIdx.x & 7, quad = threadIdx.x >> 3;
+    const uint32_t seq = blockIdx.x * 2 + r8 / kGroup;
+    const int h = r8 % kGroup;
+    if (seq >= p.batch) return;
+    Fold f;
+    {
+        const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h;
+        const uint32_t run = head * p.groups + mtile / 2;
+        const Split split(p.runs * p.tiles, p.prefix_ctas);
+        const uint32_t first = split.of(run * p.tiles), last = split.of((run + 1) * p.tiles - 1);
+        const uint32_t n = (last - first + 1) * (p.dual ? 2 : 1);
+        const float* base = p.prefix + ((size_t)(first + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
+        const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
+#pragma unroll 4
+        for (uint32_t i = 0; i < n; ++i) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(base + i * step) + quad * kTileRows + row);
+            f.add(ml.x, ml.y, v);
+        }
+    }
+    const uint32_t before = p.cum[seq], units = p.cum[seq + 1] - before;
+    if (units) {
+        const uint32_t run = seq * p.heads + head, begin = before * p.heads + head * units;
+        const Split split(p.cum[p.batch] * p.heads, p.own_ctas);
+        const uint32_t first = split.of(begin), last = split.of(begin + units - 1);
+        for (uint32_t c = first; c <= last; ++c) {
+            const float* slot = first == last ? p.whole + (size_t)run * kPartFloats
+                                              : p.part + ((size_t)c * 2 + (c == first)) * kPartFloats;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot) + h);
+            f.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(slot + 2 * kGroup + h * kDim) + quad));
+        }
+    }
+    const float inv = f.L > 0.0f ? 1.0f / f.L : (f.L == f.L ? 0.0f : f.L);
+    const __half2 a = __floats2half2_rn(f.acc.x * inv, f.acc.y * inv), b = __floats2half2_rn(f.acc.z * inv, f.acc.w * inv);
+    reinterpret_cast<uint2*>(p.out + (((size_t)seq * p.heads + head) * kGroup + h) * kDim)[quad] =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
-struct Layout {
-    size_t info, part, whole, total;
+
+struct Geometry {
+    uint32_t tiles, groups, runs;
+    bool dual;
+    size_t slots;  // of prefix partials
+    size_t cum, info, part, whole, total;
 };
-Layout layout_of(size_t batch, int heads) {
-    Layout l{};
-    l.info = align256((batch + 1) * 8);
-    l.part = l.info + align256(kAttnMaxCtas * sizeof(RunInfo));
-    l.whole = l.part + align256((size_t)kAttnMaxCtas * 2 * kPartFloats * 4);
-    l.total = l.whole + align256(batch * heads * kPartFloats * 4);
-    return l;
+Geometry geometry(size_t batch, int heads, size_t prefix_tokens) {
+    Geometry g{};
+    g.tiles = (uint32_t)((prefix_tokens + kTileTokens - 1) / kTileTokens);
+    const size_t mtiles = (batch + kTileSeqs - 1) / kTileSeqs;
+    g.dual = mtiles == 1;
+    g.groups = (uint32_t)((mtiles + 1) / 2);
+    g.runs = (uint32_t)heads * g.groups;
+    g.slots = std::min<size_t>((size_t)g.runs * g.tiles, kPrefixMaxCtas) + g.runs;
+    g.cum = align256(g.slots * 2 * kRowsFloats * 4);
+    g.info = g.cum + align256((batch + 1) * 4);
+    g.part = g.info + align256(kAttnMaxCtas * sizeof(RunInfo));
+    g.whole = g.part + align256((size_t)kAttnMaxCtas * 2 * kPartFloats * 4);
+    g.total = g.whole + align256(batch * heads * kPartFloats * 4);
+    return g;
+}
+
+template <bool kDual>
+cudaError_t launch_prefix(const PrefixParams& p, unsigned grid, cudaStream_t stream) {
+    static thread_local int configured = -1;
+    const int device = device_info().ordinal;
+    if (configured != device) {
+        cudaError_t e = cudaFuncSetAttribute(kv_prefix_kernel<kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Plan<kDual>::kSmem);
+        if (e != cudaSuccess) return e;
+        configured = device;
+    }
+    return launch_dependent(kv_prefix_kernel<kDual>, dim3(grid), dim3(kPrefixThreads), Plan<kDual>::kSmem, stream, false, p);
 }
 
 }  // namespace
@@ -75,8 +584,9 @@ using namespace hsb;
 
 extern "C" {
 
-size_t hsb_kv_attention_shared_workspace_bytes(size_t batch, int kv_heads, size_t) {
-    return 2 * layout_of(batch, kv_heads).total;
+size_t hsb_kv_attention_shared_workspace_bytes(size_t batch, int kv_heads, size_t prefix_tokens) {
+    if (!batch || batch > kMaxBatch || kv_heads < 1 || kv_heads > HSB_KV_HEADS || prefix_tokens > kMaxPrefix) return 0;
+    return geometry(batch, kv_heads, prefix_tokens).total;
 }
 
 int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_table, size_t prefix_tokens,
@@ -86,50 +596,66 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     if (!kv_pages_valid(prefix) || !kv_pages_valid(pages)) return record_error(HSB_E_KV_SHAPE, "paged KV pool arguments");
     if (prefix->format != HSB_KV_F16 || prefix->kv_heads != pages->kv_heads)
         return record_error(HSB_E_KV_SHAPE, "a shared prefix is an F16 pool of the same KV heads");
-    if (!d_prefix_table || !prefix_tokens || prefix_tokens > kMaxTableEntries || !d_table || !table_width ||
+    if (!d_prefix_table || !prefix_tokens || prefix_tokens > kMaxPrefix || !d_table || !table_width ||
         table_width > kMaxTableEntries || !d_lengths || !batch || batch > kMaxBatch ||
         batch * table_width > kMaxTableEntries || !d_q || !d_out)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
     if (((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_workspace)) & 15u) ||
         (reinterpret_cast<uintptr_t>(d_out) & 7u))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
-    if (!d_workspace || workspace_bytes < hsb_kv_attention_shared_workspace_bytes(batch, pages->kv_heads, prefix_tokens))
+    const Geometry g = geometry(batch, pages->kv_heads, prefix_tokens);
+    if ((unsigned long long)g.runs * g.tiles > 0x7fffffffull)
+        return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
+    if (!d_workspace || workspace_bytes < g.total)
         return record_error(HSB_E_WORKSPACE, "paged KV attention workspace missing or too small");
-    const Layout l = layout_of(batch, pages->kv_heads);
-    const size_t prefix_pages = (prefix_tokens + kPageTokens - 1) / kPageTokens;
+    unsigned char* ws = static_cast<unsigned char*>(d_workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+    PrefixParams p{};
+    p.v = paged_view(*prefix, d_prefix_table, (prefix_tokens + kPageTokens - 1) / kPageTokens, 0);
+    p.tokens = (uint32_t)prefix_tokens;
+    p.tiles = g.tiles;
+    p.q = d_q;
+    p.batch = (uint32_t)batch;
+    p.groups = g.groups;
+    p.runs = g.runs;
+    p.part = reinterpret_cast<float*>(ws);
+    p.status = d_status;
+    p.scale_log2 = kScaleLog2;
+    const unsigned grid = std::min<unsigned>({g.runs * g.tiles, (unsigned)device_info().sms, kPrefixMaxCtas});
+    cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
+    if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
+
+    PagedAttention a{};
+    a.v = paged_view(*pages, d_table, table_width, table_width);
+    a.lengths = d_lengths;
+    a.batch = batch;
+    a.q = d_q;
+    a.cum = reinterpret_cast<uint32_t*>(ws + g.cum);
+    a.info = reinterpret_cast<RunInfo*>(ws + g.info);
+    a.part = reinterpret_cast<float*>(ws + g.part);
+    a.whole = reinterpret_cast<float*>(ws + g.whole);
+    a.status = d_status;
+    a.scale_log2 = kScaleLog2;
+    const unsigned own = paged_attention_grid(batch * table_width * pages->kv_heads);
+    e = launch_paged_partials(pages->format, a, own, s);
+    if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
+
     SharedCombine c{};
-    for (int which = 0; which < 2; ++which) {
-        unsigned char* ws = static_cast<unsigned char*>(d_workspace) + which * l.total;
-        PagedAttention p{};
-        p.v = which ? paged_view(*pages, d_table, table_width, table_width)
-                    : paged_view(*prefix, d_prefix_table, prefix_pages, 0);
-        p.lengths = which ? d_lengths : nullptr;
-        p.length = prefix_tokens;
-        p.batch = batch;
-        p.q = d_q;
-        p.cum = reinterpret_cast<uint32_t*>(ws);
-        p.info = reinterpret_cast<RunInfo*>(ws + l.info);
-        p.part = reinterpret_cast<float*>(ws + l.part);
-        p.whole = reinterpret_cast<float*>(ws + l.whole);
-        p.status = d_status;
-        p.scale_log2 = kScaleLog2;
-        const unsigned grid = paged_attention_grid(2 * batch * pages->kv_heads * p.v.width);
-        cudaError_t e = launch_paged_partials(which ? pages->format : HSB_KV_F16, p, grid, s);
-        if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
-        Source& src = which ? c.own : c.prefix;
-        src.part = p.part;
-        src.whole = p.whole;
-        src.units = which ? 0 : batch * pages->kv_heads * ((prefix_tokens + 31) / 32);
-        src.ctas = grid;
-        c.cum = p.cum;
-    }
-    c.prefix_units = (prefix_tokens + 31) / 32;
-    c.batch = batch;
+    c.prefix = p.part;
+    c.tiles = g.tiles;
+    c.groups = g.groups;
+    c.runs = g.runs;
+    c.prefix_ctas = grid;
+    c.dual = g.dual;
+    c.part = a.part;
+    c.whole = a.whole;
+    c.cum = a.cum;
+    c.own_ctas = own;
+    c.batch = (uint32_t)batch;
     c.heads = pages->kv_heads;
     c.out = d_out;
-    cudaError_t e = launch_dependent(kv_shared_combine_kernel, dim3((unsigned)(batch * pages->kv_heads)),
-                                     dim3(kGroup * kDim), 0, s, false, c);
+    e = launch_dependent(kv_shared_combine_kernel, dim3((unsigned)((batch + 1) / 2), pages->kv_heads), dim3(256), 0, s, false, c);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
     record_error(HSB_OK, "");
     return HSB_OK;
