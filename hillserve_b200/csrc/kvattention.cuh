@@ -5,7 +5,7 @@
 
 namespace hsb {
 
-constexpr unsigned kAttnMaxCtas = 512;
+constexpr unsigned kAttnMaxCtas = 160;
 constexpr int kPartFloats = kGroup * 2 + kGroup * kDim;  // (max in log2 units, sum) per head, then the outputs
 constexpr size_t kMaxBatch = 1u << 20;
 constexpr size_t kMaxTableEntries = 1ull << 27;  // keeps the units of 8 heads within 32 bits

@@ -33,9 +33,9 @@ constexpr int kTileSeqs = kTileRows / kGroup;
 constexpr int kTileBytes = kTileTokens * 256;       // K or V of a tile; also a Q tile
 constexpr int kTilePanel = kTileTokens * 128;       // its 64-channel half
 constexpr int kSoftmaxThreads = 256;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kPrefixThreads = 320;
-constexpr unsigned kPrefixMaxCtas = 160;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;          // of a third warpgroup, which gives its registers
+constexpr int kPrefixThreads = 384;                 // to the other two (setmaxnreg)
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr float kSlack = 8.0f;                      // weights are at most 2^8 (F16 holds 2^15)
 constexpr int kLive = 16;                           // ring of tiles' live counts
 // a partial: outputs [32 channel quads][128 rows][4], then (max, sum) [128 rows]
@@ -125,8 +125,67 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 // Generic writes to shared memory before the tensor cores or bulk copies use it.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---------------------------------------------------------------- softmax
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Two F32 values in a register pair, and the paired operations.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void split_of(uint64_t d, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// One pair of kByPolynomial takes its powers of two from the FMA units, as the
+// special-function unit alone (16 a clock) would take as long as the products:
+// 2^y = 2^n 2^f with n the nearest integer (adding 1.5 2^23 rounds to it) and
+// 2^f on [-0.5, 0.5] a polynomial of degree 4, fitted for the least largest
+// relative error (2.7e-6; a weight is rounded to F16 by 5e-4 next).
+#ifndef BYPOLY
+#define BYPOLY 4
+#endif
+constexpr int kByPolynomial = BYPOLY;
+__device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
+    constexpr float kRound = 12582912.0f;
+    float ya, yb;
+    split_of(y2, ya, yb);
+    const uint64_t y = pair_of(fmaxf(ya, -126.0f), fmaxf(yb, -126.0f));  // (-infinity too: 2^-126 is 0 in F16)
+    const uint64_t t = add2(y, pair_of(kRound, kRound));
+    const uint64_t f = add2(y, fma2(t, pair_of(-1.0f, -1.0f), pair_of(kRound, kRound)));
+    uint64_t v = pair_of(0.0095701013f, 0.0095701013f);
+    v = fma2(v, f, pair_of(0.0559178591f, 0.0559178591f));
+    v = fma2(v, f, pair_of(0.2402474433f, 0.2402474433f));
+    v = fma2(v, f, pair_of(0.6931217909f, 0.6931217909f));
+    v = fma2(v, f, pair_of(0.9999992847f, 0.9999992847f));
+    float ta, tb, va, vb;
+    split_of(t, ta, tb);
+    split_of(v, va, vb);
+    a = __uint_as_float(__float_as_uint(va) + (__float_as_uint(ta) << 23));
+    b = __uint_as_float(__float_as_uint(vb) + (__float_as_uint(tb) << 23));
+}
 
 // Waits for a phase; gives up after kWaitLimitNs or once another role did.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -155,7 +214,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     using P = Plan<kDual>;
     constexpr int kStages = P::kStages;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2];
+    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], cleaned, last;
     __shared__ uint32_t tmem_s;
     __shared__ int live_s[kLive][2];  // tokens of a tile's two pages that count
     __shared__ volatile int dead;
@@ -168,6 +227,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             mbar_init(&empty[i], 1);
         }
         mbar_init(&q_full, kSoftmaxThreads);
+        mbar_init(&cleaned, 1);
+        mbar_init(&last, 1);
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
             mbar_init(&p_full[w], 128);
@@ -186,167 +247,186 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     const Split split(p.runs * p.tiles, gridDim.x);
     Segment seg{split.begin(blockIdx.x), split.begin(blockIdx.x + 1), p.tiles};
 
-    if (warp == kLoadWarp) {
-        // ================ loader: K and V tiles in the order the products take them
-        uint32_t it = 0;
-        bool ok = true;
-        const auto load = [&](uint32_t tile, int head, int part, uint32_t number) {
-            const uint32_t s = it % kStages;
-            if (it >= (uint32_t)kStages) ok = ok && __all_sync(0xffffffffu, wait_phase(&empty[s], ((it / kStages) - 1) & 1, &dead));
-            if (!ok) return;
-            const uint32_t token = tile * kTileTokens + (lane & 1) * kPageTokens;
-            int32_t id = -1;
-            int live = 0;
-            if (lane < 2 && token < p.tokens) {
-                id = p.v.table[token / kPageTokens];
-                if (id < 0 || (unsigned long long)id >= p.v.pages) {
-                    id = -1;  // no such page: its tokens are left out
-                    if (part == 0) raise_status(p.status, HSB_E_KV_PAGE, 0);
+    if (warp >= kSoftmaxThreads / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp) {
+            // ================ loader: K and V tiles in the order the products take them
+            uint32_t it = 0;
+            bool ok = true;
+            uint32_t ids_first = 0;  // this lane's page of the 16 tiles from there: its id and tokens
+            int32_t id32 = -1;
+            int live32 = 0;
+            const auto look_up = [&](uint32_t tile) {
+                ids_first = tile;
+                const uint32_t token = tile * kTileTokens + lane * kPageTokens;
+                id32 = -1;
+                live32 = 0;
+                if (token >= p.tokens) return;
+                id32 = p.v.table[token / kPageTokens];
+                if (id32 < 0 || (unsigned long long)id32 >= p.v.pages) {
+                    id32 = -1;  // no such page: its tokens are left out
+                    raise_status(p.status, HSB_E_KV_PAGE, 0);
                 } else {
-                    live = (int)min(p.tokens - token, (uint32_t)kPageTokens);
+                    live32 = (int)min(p.tokens - token, (uint32_t)kPageTokens);
                 }
-            }
-            if (lane < 2 && part == 0) live_s[number % kLive][lane] = live;
-            const unsigned have = __ballot_sync(0xffffffffu, id >= 0);
-            __syncwarp();
-            if (lane == 0) {
-                if (have) mbar_arrive_expect_tx(&full[s], __popc(have) * 2 * kPanelBytes);
-                else mbar_arrive(&full[s]);
-            }
-            __syncwarp();
-            if (id >= 0) {
-                const unsigned char* src = p.v.data + ((size_t)id * p.v.heads + head) * PageFormat<HSB_KV_F16>::kBytes;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    bulk_copy_g2s(smem + P::kQBytes + s * kTileBytes + i * kTilePanel + lane * kPanelBytes,
-                                  src + (part * 2 + i) * kPanelBytes, kPanelBytes, &full[s]);
-            }
-            __syncwarp();
-            ++it;
-        };
-        uint32_t number = 0;  // tiles of earlier segments
-        for (; ok && !seg.done(); seg.next()) {
-            const int head = (int)(seg.run() / p.groups);
-            const uint32_t first = seg.first(), n = seg.count();
-            load(first, head, 0, number);
-            for (uint32_t i = 0; ok && i < n; ++i) {
-                if (kDual && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
-                if (ok) load(first + i, head, 1, number + i);
-                if (!kDual && ok && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
-            }
-            number += n;
-        }
-        if (!ok) {  // copies in flight land before shared memory is released
-            const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0;
-            for (uint32_t j = from; j < it; ++j) (void)mbar_wait(&full[j % kStages], (j / kStages) & 1);
-        }
-    } else if (warp == kMmaWarp) {
-        // ================ products
-        uint32_t it = 0, number = 0, segment = 0, weights[2] = {0, 0};
-        bool ok = true;
-        const auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && __all_sync(0xffffffffu, wait_phase(bar, parity, &dead));
-        };
-        const auto take = [&]() {  // the next stage, filled
-            const uint32_t s = it % kStages;
-            wait_all(&full[s], (it / kStages) & 1);
-            ++it;
-            return s;
-        };
-        const auto logits = [&](int w, uint32_t s) {
-            if (ok && lane == 0) {
-                const uint32_t a = q_s + (kDual ? 0 : w * kTileBytes), b = ring_s + s * kTileBytes;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t at = (k >> 2) * kTilePanel + (k & 3) * 32;
-                    tc_mma(tmem + w * 128, operand(a + at, 16), operand(b + at, 16), kShapeK, k > 0);
+            };
+            const auto load = [&](uint32_t tile, int head, int part, uint32_t number) {
+                const uint32_t s = it % kStages;
+                if (it >= (uint32_t)kStages) ok = ok && __all_sync(0xffffffffu, wait_phase(&empty[s], ((it / kStages) - 1) & 1, &dead));
+                if (!ok) return;
+                const int from = (int)(tile - ids_first) * 2 + (lane & 1);
+                const int32_t id = __shfl_sync(0xffffffffu, id32, from);
+                const int live = __shfl_sync(0xffffffffu, live32, from);
+                if (lane < 2 && part == 0) live_s[number % kLive][lane] = live;
+                const unsigned have = __ballot_sync(0xffffffffu, lane < 2 && id >= 0);
+                __syncwarp();
+                if (lane == 0) {
+                    if (have) mbar_arrive_expect_tx(&full[s], __popc(have) * 2 * kPanelBytes);
+                    else mbar_arrive(&full[s]);
                 }
-                tc_commit(&s_full[w]);
-            }
-            __syncwarp();
-        };
-        const auto output = [&](int w, uint32_t s, bool add) {
-            wait_all(&p_full[w], weights[w]++ & 1);
-            tc_fence_after();
-            if (ok && lane == 0) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + k * 8,
-                                operand(ring_s + s * kTileBytes + k * 16 * 128, kTilePanel), kShapeMN, add || k > 0);
-            }
-            __syncwarp();
-        };
-        // rows of V behind the last token (or of a page that is not there) may hold NaN: zero them
-        const auto clean = [&](uint32_t s, uint32_t tile_number) {
-            if (!ok) return;
-            const int l0 = live_s[tile_number % kLive][0], l1 = live_s[tile_number % kLive][1];
-            if (l0 == kPageTokens && l1 == kPageTokens) return;
-            for (int i = lane; i < kTileTokens * 16; i += 32) {
-                const int row = i >> 4, c = i & 15;
-                if (row < kPageTokens ? row >= l0 : row - kPageTokens >= l1)
-                    *reinterpret_cast<uint4*>(smem + P::kQBytes + s * kTileBytes + (c >> 3) * kTilePanel + row * 128 +
-                                              (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_shared();
-            __syncwarp();
-        };
-        const auto commit = [&](uint64_t* bar) {
-            if (ok && lane == 0) tc_commit(bar);
-            __syncwarp();
-        };
-        for (; ok && !seg.done(); seg.next(), ++segment) {
-            const uint32_t n = seg.count();
-            wait_all(&q_full, segment & 1);
-            tc_fence_after();
-            if constexpr (kDual) {
-                for (uint32_t i = 0; i < 2 && i < n; ++i) {
-                    const uint32_t s = take();
-                    logits(i, s);
-                    commit(&empty[s]);
+                __syncwarp();
+                if (lane < 2 && id >= 0) {
+                    const unsigned char* src = p.v.data + ((size_t)id * p.v.heads + head) * PageFormat<HSB_KV_F16>::kBytes;
+    #pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        bulk_copy_g2s(smem + P::kQBytes + s * kTileBytes + i * kTilePanel + lane * kPanelBytes,
+                                      src + (part * 2 + i) * kPanelBytes, kPanelBytes, &full[s]);
                 }
-                for (uint32_t i = 0; ok && i < n; ++i) {
-                    const int w = i & 1;
-                    const uint32_t s = take();
-                    clean(s, number + i);
-                    output(w, s, i >= 2);
-                    commit(&empty[s]);
-                    if (i + 2 < n) {
-                        const uint32_t next = take();
-                        logits(w, next);
-                        commit(&empty[next]);
-                    } else {
-                        commit(&o_full[w]);
+                __syncwarp();
+                const uint32_t parity = (it++ / kStages) & 1;
+                // rows of V behind the last token (or of a page that is not there) may hold NaN: zero them
+                const int l0 = __shfl_sync(0xffffffffu, live, 0), l1 = __shfl_sync(0xffffffffu, live, 1);
+                if (part && l0 + l1 < kTileTokens) {
+                    ok = ok && __all_sync(0xffffffffu, wait_phase(&full[s], parity, &dead));
+                    for (int i = lane; i < kTileTokens * 16; i += 32) {
+                        const int r = i >> 4, c = i & 15;
+                        if (r < kPageTokens ? r >= l0 : r - kPageTokens >= l1)
+                            *reinterpret_cast<uint4*>(smem + P::kQBytes + s * kTileBytes + (c >> 3) * kTilePanel + r * 128 +
+                                                      (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&cleaned);
                 }
-                if (n == 1) commit(&o_full[1]);
-            } else {
-                uint32_t s = take();
-                logits(0, s);
-                logits(1, s);
-                commit(&empty[s]);
+            };
+            uint32_t number = 0;  // tiles of earlier segments
+            for (; ok && !seg.done(); seg.next()) {
+                const int head = (int)(seg.run() / p.groups);
+                const uint32_t first = seg.first(), n = seg.count();
+                look_up(first);
+                load(first, head, 0, number);
                 for (uint32_t i = 0; ok && i < n; ++i) {
-                    const uint32_t v = take();
-                    clean(v, number + i);
-                    output(0, v, i > 0);
-                    if (i + 1 < n) {
-                        s = take();
+                    if (first + i + 1 >= ids_first + 16) look_up(first + i);
+                    if (kDual && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
+                    if (ok) load(first + i, head, 1, number + i);
+                    if (!kDual && ok && i + 1 < n) load(first + i + 1, head, 0, number + i + 1);
+                }
+                number += n;
+            }
+            if (!ok) {  // copies in flight land before shared memory is released
+                const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0;
+                for (uint32_t j = from; j < it; ++j) (void)mbar_wait(&full[j % kStages], (j / kStages) & 1);
+            }
+        } else if (warp == kMmaWarp) {
+            // ================ products: one thread issues them all
+            if (elect_one()) {
+                uint32_t it = 0, number = 0, segment = 0, weights[2] = {0, 0}, cleanings = 0;
+                bool ok = true;
+                const uint64_t q_desc = operand(q_s, 16), k_desc = operand(ring_s, 16), v_desc = operand(ring_s, kTilePanel);
+                const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && wait_phase(bar, parity, &dead); };
+                const auto take = [&]() {  // the next stage, filled
+                    const uint32_t s = it % kStages;
+                    wait(&full[s], (it / kStages) & 1);
+                    ++it;
+                    return s;
+                };
+                const auto logits = [&](int w, uint32_t s) {
+                    if (!ok) return;
+                    const uint64_t a = q_desc + (kDual ? 0 : w * (kTileBytes >> 4)), b = k_desc + s * (kTileBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int at = ((k >> 2) * kTilePanel + (k & 3) * 32) >> 4;
+                        tc_mma(tmem + w * 128, a + at, b + at, kShapeK, k > 0);
+                    }
+                    tc_commit(&s_full[w]);
+                };
+                const auto output = [&](int w, uint32_t s, bool add) {
+                    wait(&p_full[w], weights[w]++ & 1);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint64_t b = v_desc + s * (kTileBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + k * 8, b + ((k * 16 * 128) >> 4), kShapeMN, add || k > 0);
+                };
+                const auto take_v = [&](uint32_t tile_number) {
+                    const uint32_t s = take();
+                    if (live_s[tile_number % kLive][0] + live_s[tile_number % kLive][1] < kTileTokens)
+                        wait(&cleaned, cleanings++ & 1);
+                    return s;
+                };
+                const auto commit = [&](uint64_t* bar) {
+                    if (ok) tc_commit(bar);
+                };
+                for (; ok && !seg.done(); seg.next(), ++segment) {
+                    const uint32_t n = seg.count();
+                    wait(&q_full, segment & 1);
+                    tc_fence_after();
+                    if constexpr (kDual) {
+                        for (uint32_t i = 0; i < 2 && i < n; ++i) {
+                            const uint32_t s = take();
+                            logits(i, s);
+                            commit(&empty[s]);
+                        }
+                        for (uint32_t i = 0; ok && i < n; ++i) {
+                            const int w = i & 1;
+                            const uint32_t s = take_v(number + i);
+                            output(w, s, i >= 2);
+                            commit(&empty[s]);
+                            if (i + 2 < n) {
+                                const uint32_t next = take();
+                                logits(w, next);
+                                commit(&empty[next]);
+                            } else {
+                                commit(&o_full[w]);
+                            }
+                        }
+                        if (n == 1) commit(&o_full[1]);
+                    } else {
+                        uint32_t s = take();
                         logits(0, s);
-                    } else {
-                        commit(&o_full[0]);
-                    }
-                    output(1, v, i > 0);
-                    commit(&empty[v]);
-                    if (i + 1 < n) {
                         logits(1, s);
                         commit(&empty[s]);
-                    } else {
-                        commit(&o_full[1]);
+                        for (uint32_t i = 0; ok && i < n; ++i) {
+                            const uint32_t v = take_v(number + i);
+                            output(0, v, i > 0);
+                            if (i + 1 < n) {
+                                s = take();
+                                logits(0, s);
+                            } else {
+                                commit(&o_full[0]);
+                            }
+                            output(1, v, i > 0);
+                            commit(&empty[v]);
+                            if (i + 1 < n) {
+                                logits(1, s);
+                                commit(&empty[s]);
+                            } else {
+                                commit(&o_full[1]);
+                            }
+                        }
                     }
+                    number += n;
+                }
+                if (!ok) {  // products in flight end before tensor memory is freed
+                    tc_commit(&last);
+                    (void)mbar_wait(&last, 0);
                 }
             }
-            number += n;
+            __syncwarp();
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ================ softmax: warpgroup w, thread = row
         const int w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -358,16 +438,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             const int head = (int)(run / p.groups);
             const uint32_t mtile = (run % p.groups) * 2;
             // ---- Q into its operand layout (the products of the last segment are done: o_full)
-            for (int i = 0; i < (kDual ? 8 : 16); ++i) {
-                const int at = kDual ? i * 256 + tid : i * 128 + row;
-                const int r = at >> 4, c = at & 15;
+            constexpr int kLoads = kDual ? 8 : 16;
+            uint4 x4[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = kDual ? i * 256 + tid : i * 128 + row, r = at >> 4, c = at & 15;
                 const uint32_t seq = (mtile + (kDual ? 0 : w)) * kTileSeqs + r / kGroup;
-                uint4 x = make_uint4(0, 0, 0, 0);  // rows behind the batch
+                x4[i] = make_uint4(0, 0, 0, 0);  // rows behind the batch
                 if (seq < p.batch)
-                    x = *reinterpret_cast<const uint4*>(
+                    x4[i] = *reinterpret_cast<const uint4*>(
                         p.q + (((size_t)seq * p.v.heads + head) * kGroup + r % kGroup) * kDim + c * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = kDual ? i * 256 + tid : i * 128 + row, r = at >> 4, c = at & 15;
                 *reinterpret_cast<uint4*>(smem + (kDual ? 0 : w * kTileBytes) + (c >> 3) * kTilePanel + r * 128 +
-                                          (((c & 7) ^ (r & 7)) << 4)) = x;
+                                          (((c & 7) ^ (r & 7)) << 4)) = x4[i];
             }
             fence_async_shared();
             mbar_arrive(&q_full);
@@ -387,9 +473,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     for (int j = 0; j < kTileTokens; ++j)
                         if (j < kPageTokens ? j >= l0 : j - kPageTokens >= l1) x[j] = -INFINITY;
                 }
-                float top = x[0];
+                float tops[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int j = 1; j < kTileTokens; ++j) top = fmaxf(top, x[j]);
+                for (int j = 4; j < kTileTokens; j += 8) {
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4)
+                        tops[i4] = j + 4 + i4 < kTileTokens ? max3(tops[i4], x[j + i4], x[j + 4 + i4]) : fmaxf(tops[i4], x[j + i4]);
+                }
+                float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
                 top *= p.scale_log2;
                 if (__any_sync(0xffffffffu, top > m + kSlack)) {
                     const float to = fmaxf(m, top);
@@ -409,17 +500,27 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
+                const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), minus2 = pair_of(-base, -base);
+                uint64_t sum2[2] = {0, 0};
                 uint32_t h[kTileTokens / 2];
-                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < kTileTokens; j += 2) {
-                    const float a = exp2_ftz(fmaf(x[j], p.scale_log2, -base));
-                    const float b = exp2_ftz(fmaf(x[j + 1], p.scale_log2, -base));
-                    sums[(j >> 1) & 3] += a + b;
+                    const uint64_t y = fma2(pair_of(x[j], x[j + 1]), scale2, minus2);
+                    float a, b;
+                    if ((j >> 1) % kByPolynomial == 0) {
+                        exp2_pair(y, a, b);
+                    } else {
+                        split_of(y, a, b);
+                        a = exp2_ftz(a);
+                        b = exp2_ftz(b);
+                    }
+                    sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pair_of(a, b));
                     const __half2 pair = __floats2half2_rn(a, b);
                     h[j >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
                 }
-                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                float la, lb;
+                split_of(add2(sum2[0], sum2[1]), la, lb);
+                l += la + lb;
                 tmem_store32(s_at, h);
                 tmem_store32(s_at + 32, h + 32);
                 tmem_wait_store();
@@ -455,15 +556,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     if (tid == 0 && dead) raise_status(p.status, HSB_E_TIMEOUT, blockIdx.x);
     tc_fence_after();
     if (warp == kMmaWarp) {
-        if (dead) {  // products in flight end before tensor memory is freed
-            if (lane == 0) {
-                mbar_init(&q_full, 1);
-                mbar_fence_init();
-                tc_commit(&q_full);
-                (void)mbar_wait(&q_full, 0);
-            }
-            __syncwarp();
-        }
         tmem_free(tmem, 512);
     }
 }
@@ -485,57 +577,112 @@ struct SharedCombine {
     uint16_t* out;
 };
 
-struct Fold {
-    float M = -INFINITY, L = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    __device__ void add(float m, float l, float4 v) {
-        if (m == -INFINITY && l == l) return;  // no token (a NaN sum comes through)
-        const float top = fmaxf(M, m);
-        const float a = M == -INFINITY ? 0.0f : exp2_ftz(M - top), b = top == -INFINITY ? 1.0f : exp2_ftz(m - top);
-        L = L * a + l * b;
-        acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
-        M = top;
-    }
-};
-
-// CTA = (two sequences, KV head): thread = (row of the two sequences' eight, channel quad).
+// CTA = (two sequences' eight rows, KV head, 128 / kSplit channels).  First the
+// weights of all partials of each row, then the sums: thread = (row, channel
+// quad), every kSplit-th partial.  kSplit 4 where the rows alone are too few
+// CTAs to keep the loads of some forty partials a row in flight.
+constexpr int kMaxParts = 3 * kAttnMaxCtas;
+template <int kSplit>
 __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
+    __shared__ float weight[kMaxParts][8];
+    __shared__ float red[8][8], inv_s[8];
+    __shared__ float4 acc_s[kSplit == 1 ? 1 : 256];
     pdl_wait();
     pdl_trigger();
-    const int head = blockIdx.y, r8 = threadIdx.x & 7, quad = threadIdx.x >> 3;
+    const int tid = threadIdx.x, head = blockIdx.y, r8 = tid & 7, warp = tid >> 5;
     const uint32_t seq = blockIdx.x * 2 + r8 / kGroup;
     const int h = r8 % kGroup;
-    if (seq >= p.batch) return;
-    Fold f;
-    {
-        const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h;
-        const uint32_t run = head * p.groups + mtile / 2;
-        const Split split(p.runs * p.tiles, p.prefix_ctas);
-        const uint32_t first = split.of(run * p.tiles), last = split.of((run + 1) * p.tiles - 1);
-        const uint32_t n = (last - first + 1) * (p.dual ? 2 : 1);
-        const float* base = p.prefix + ((size_t)(first + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
-        const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
-#pragma unroll 4
-        for (uint32_t i = 0; i < n; ++i) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(base + i * step) + quad * kTileRows + row);
-            f.add(ml.x, ml.y, v);
+    const bool there = seq < p.batch;
+    // the row's partials: `n` of the prefix, `m` of its own tokens
+    const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h, run = head * p.groups + mtile / 2;
+    const Split prefix(p.runs * p.tiles, p.prefix_ctas);
+    const uint32_t p0 = prefix.of(run * p.tiles), p1 = prefix.of((run + 1) * p.tiles - 1);
+    const uint32_t n = (p1 - p0 + 1) * (p.dual ? 2 : 1);
+    const float* base = p.prefix + ((size_t)(p0 + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
+    const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
+    uint32_t m = 0, c0 = 0;
+    const float* own = nullptr;
+    if (there) {
+        const uint32_t before = p.cum[seq], units = p.cum[seq + 1] - before, all = p.cum[p.batch];
+        if (units) {
+            const uint32_t begin = before * p.heads + head * units;
+            const Split split(all * p.heads, p.own_ctas);
+            c0 = split.of(begin);
+            m = split.of(begin + units - 1) - c0 + 1;
+            own = m == 1 ? p.whole + ((size_t)seq * p.heads + head) * kPartFloats : p.part + (size_t)c0 * 2 * kPartFloats;
         }
     }
-    const uint32_t before = p.cum[seq], units = p.cum[seq + 1] - before;
-    if (units) {
-        const uint32_t run = seq * p.heads + head, begin = before * p.heads + head * units;
-        const Split split(p.cum[p.batch] * p.heads, p.own_ctas);
-        const uint32_t first = split.of(begin), last = split.of(begin + units - 1);
-        for (uint32_t c = first; c <= last; ++c) {
-            const float* slot = first == last ? p.whole + (size_t)run * kPartFloats
-                                              : p.part + ((size_t)c * 2 + (c == first)) * kPartFloats;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot) + h);
-            f.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(slot + 2 * kGroup + h * kDim) + quad));
+    const auto own_at = [&](uint32_t i) { return own + (m == 1 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
+    // ---- weights: 32 partials at a time
+    const uint32_t total = there ? n + m : 0;
+    float l[(kMaxParts + 31) / 32], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < (kMaxParts + 31) / 32; ++k) {
+        const uint32_t i = k * 32 + (tid >> 3);
+        if (i >= total) break;
+        const float2 ml = i < n ? __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row)
+                                : __ldcg(reinterpret_cast<const float2*>(own_at(i - n)) + h);
+        weight[i][r8] = ml.x;
+        l[k] = ml.y;
+        top = fmaxf(top, ml.x);
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    if ((tid & 31) < 8) red[warp][r8] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w][r8]);
+    __syncthreads();
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < (kMaxParts + 31) / 32; ++k) {
+        const uint32_t i = k * 32 + (tid >> 3);
+        if (i >= total) break;
+        // (all -infinity: no token, sums 0; a NaN sum comes through)
+        const float f = top == -INFINITY ? 1.0f : exp2_ftz(weight[i][r8] - top);
+        weight[i][r8] = f;
+        sum = fmaf(f, l[k], sum);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    if ((tid & 31) < 8) red[warp][r8] = sum;
+    __syncthreads();
+    if (tid < 8) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += red[w][r8];
+        inv_s[r8] = s > 0.0f ? 1.0f / s : (s == s ? 0.0f : s);
+    }
+    __syncthreads();
+    // ---- sums
+    const int quad = kSplit == 1 ? tid >> 3 : blockIdx.z * (32 / kSplit) + (tid >> 3) % (32 / kSplit);
+    const uint32_t part = kSplit == 1 ? 0 : (tid >> 3) / (32 / kSplit);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](uint32_t i, float4 v) {
+        const float f = weight[i][r8];
+        acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
+    };
+    if (there) {
+        uint32_t i = part;
+        const float4* at = reinterpret_cast<const float4*>(base) + quad * kTileRows + row;
+#pragma unroll 8
+        for (; i < n; i += kSplit) add(i, __ldcg(at + i * step / 4));
+        for (; i < total; i += kSplit)
+            add(i, __ldcg(reinterpret_cast<const float4*>(own_at(i - n) + 2 * kGroup + h * kDim) + quad));
+    }
+    if constexpr (kSplit > 1) {
+        acc_s[tid] = acc;
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int k = 1; k < kSplit; ++k) {
+            const float4 v = acc_s[tid + k * (256 / kSplit)];
+            acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
         }
     }
-    const float inv = f.L > 0.0f ? 1.0f / f.L : (f.L == f.L ? 0.0f : f.L);
-    const __half2 a = __floats2half2_rn(f.acc.x * inv, f.acc.y * inv), b = __floats2half2_rn(f.acc.z * inv, f.acc.w * inv);
+    if (!there) return;
+    const float inv = inv_s[r8];
+    const __half2 a = __floats2half2_rn(acc.x * inv, acc.y * inv), b = __floats2half2_rn(acc.z * inv, acc.w * inv);
     reinterpret_cast<uint2*>(p.out + (((size_t)seq * p.heads + head) * kGroup + h) * kDim)[quad] =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
@@ -555,7 +702,7 @@ Geometry geometry(size_t batch, int heads, size_t prefix_tokens) {
     g.dual = mtiles == 1;
     g.groups = (uint32_t)((mtiles + 1) / 2);
     g.runs = (uint32_t)heads * g.groups;
-    g.slots = std::min<size_t>((size_t)g.runs * g.tiles, kPrefixMaxCtas) + g.runs;
+    g.slots = std::min<size_t>((size_t)g.runs * g.tiles, kAttnMaxCtas) + g.runs;
     g.cum = align256(g.slots * 2 * kRowsFloats * 4);
     g.info = g.cum + align256((batch + 1) * 4);
     g.part = g.info + align256(kAttnMaxCtas * sizeof(RunInfo));
@@ -569,8 +716,12 @@ cudaError_t launch_prefix(const PrefixParams& p, unsigned grid, cudaStream_t str
     static thread_local int configured = -1;
     const int device = device_info().ordinal;
     if (configured != device) {
-        cudaError_t e = cudaFuncSetAttribute(kv_prefix_kernel<kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Plan<kDual>::kSmem);
+        cudaFuncAttributes attr{};
+        cudaError_t e = cudaFuncGetAttributes(&attr, kv_prefix_kernel<kDual>);
+        if (e != cudaSuccess) return e;
+        // the warpgroups' shares are drawn from what the block was launched with: more would wait for ever
+        if (attr.numRegs * kPrefixThreads < 128 * (2 * kSoftmaxRegs + kOtherRegs)) return cudaErrorLaunchOutOfResources;
+        e = cudaFuncSetAttribute(kv_prefix_kernel<kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<kDual>::kSmem);
         if (e != cudaSuccess) return e;
         configured = device;
     }
@@ -622,7 +773,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     p.part = reinterpret_cast<float*>(ws);
     p.status = d_status;
     p.scale_log2 = kScaleLog2;
-    const unsigned grid = std::min<unsigned>({g.runs * g.tiles, (unsigned)device_info().sms, kPrefixMaxCtas});
+    const unsigned grid = std::min<unsigned>({g.runs * g.tiles, (unsigned)device_info().sms, kAttnMaxCtas});
     cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
 
@@ -655,7 +806,11 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.batch = (uint32_t)batch;
     c.heads = pages->kv_heads;
     c.out = d_out;
-    e = launch_dependent(kv_shared_combine_kernel, dim3((unsigned)((batch + 1) / 2), pages->kv_heads), dim3(256), 0, s, false, c);
+    const dim3 rows((unsigned)((batch + 1) / 2), pages->kv_heads);
+    if (rows.x * rows.y < 2u * device_info().sms)
+        e = launch_dependent(kv_shared_combine_kernel<4>, dim3(rows.x, rows.y, 4), dim3(256), 0, s, false, c);
+    else
+        e = launch_dependent(kv_shared_combine_kernel<1>, rows, dim3(256), 0, s, false, c);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
     record_error(HSB_OK, "");
     return HSB_OK;
