@@ -234,7 +234,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         mbar_fence_init();
         pieces[warp][0].there = pieces[warp][1].there = 0;
     }
-    pdl_wait();
+    // Partial mode follows kv_prefix_kernel, which lets this grid start only once everything
+    // before itself is complete, and whose results are not read here: only the end waits, so
+    // that what follows finds both.
+    if (kFinal) pdl_wait();
     pdl_trigger();
     uint32_t units, stretch[2];
     Walker<R> k = find_part<R>(p, &units, stretch);
@@ -250,7 +253,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         info.run = -1;
         p.info[blockIdx.x] = info;
     }
-    if (stretch[0] >= stretch[1]) return;
+    if (stretch[0] >= stretch[1]) {
+        if (!kFinal) pdl_wait();
+        return;
+    }
 
     const int g = lane >> 2, t = lane & 3;
     // this lane's share of a run's query head g & 3: for step ks the channels of its K words
@@ -642,6 +648,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             open = -1;
         }
     }
+    if (!kFinal) pdl_wait();
 }
 
 // Folds the partials of the run that begins in CTA blockIdx.x's stretch and

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     using P = Plan<kDual>;
     constexpr int kStages = P::kStages;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2], o_full[2], cleaned, last;
+    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], o_full[2], cleaned, last;
     __shared__ uint32_t tmem_s;
     __shared__ int live_s[kLive][2];  // tokens of a tile's two pages that count
     __shared__ volatile int dead;
@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
         mbar_init(&last, 1);
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
-            mbar_init(&p_full[w], 128);
+            mbar_init(&p_full[w][0], 128);
+            mbar_init(&p_full[w][1], 128);
             mbar_init(&o_full[w], 1);
         }
         mbar_fence_init();
@@ -351,13 +352,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     tc_commit(&s_full[w]);
                 };
                 const auto output = [&](int w, uint32_t s, bool add) {
-                    wait(&p_full[w], weights[w]++ & 1);
-                    if (!ok) return;
-                    tc_fence_after();
                     const uint64_t b = v_desc + s * (kTileBytes >> 4);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + k * 8, b + ((k * 16 * 128) >> 4), kShapeMN, add || k > 0);
+                    for (int half = 0; half < 2; ++half) {  // the first 64 tokens' while the others' weights are made
+                        wait(&p_full[w][half], weights[w] & 1);
+                        if (!ok) return;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = half * 4; k < half * 4 + 4; ++k)
+                            tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + k * 8, b + ((k * 16 * 128) >> 4), kShapeMN,
+                                        add || k > 0);
+                    }
+                    ++weights[w];
                 };
                 const auto take_v = [&](uint32_t tile_number) {
                     const uint32_t s = take();
@@ -502,30 +508,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                 const float base = m == -INFINITY ? 0.0f : m;
                 const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), minus2 = pair_of(-base, -base);
                 uint64_t sum2[2] = {0, 0};
-                uint32_t h[kTileTokens / 2];
 #pragma unroll
-                for (int j = 0; j < kTileTokens; j += 2) {
-                    const uint64_t y = fma2(pair_of(x[j], x[j + 1]), scale2, minus2);
-                    float a, b;
-                    if ((j >> 1) % kByPolynomial == 0) {
-                        exp2_pair(y, a, b);
-                    } else {
-                        split_of(y, a, b);
-                        a = exp2_ftz(a);
-                        b = exp2_ftz(b);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t h[kTileTokens / 4];
+#pragma unroll
+                    for (int j = 0; j < kTileTokens / 2; j += 2) {
+                        const int at = half * (kTileTokens / 2) + j;
+                        const uint64_t y = fma2(pair_of(x[at], x[at + 1]), scale2, minus2);
+                        float a, b;
+                        if ((j >> 1) % kByPolynomial == 0) {
+                            exp2_pair(y, a, b);
+                        } else {
+                            split_of(y, a, b);
+                            a = exp2_ftz(a);
+                            b = exp2_ftz(b);
+                        }
+                        sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pair_of(a, b));
+                        const __half2 pair = __floats2half2_rn(a, b);
+                        h[j >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
                     }
-                    sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pair_of(a, b));
-                    const __half2 pair = __floats2half2_rn(a, b);
-                    h[j >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
+                    tmem_store32(s_at + half * 32, h);
+                    tmem_wait_store();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[w][half]);
                 }
                 float la, lb;
                 split_of(add2(sum2[0], sum2[1]), la, lb);
                 l += la + lb;
-                tmem_store32(s_at, h);
-                tmem_store32(s_at + 32, h + 32);
-                tmem_wait_store();
-                tc_fence_before();
-                mbar_arrive(&p_full[w]);
             }
             // ---- the segment's partial
             if (ok) ok = __all_sync(0xffffffffu, wait_phase(&o_full[w], segment & 1, &dead));
@@ -577,22 +586,21 @@ struct SharedCombine {
     uint16_t* out;
 };
 
-// CTA = (two sequences' eight rows, KV head, 128 / kSplit channels).  First the
-// weights of all partials of each row, then the sums: thread = (row, channel
-// quad), every kSplit-th partial.  kSplit 4 where the rows alone are too few
-// CTAs to keep the loads of some forty partials a row in flight.
+// CTA = (two sequences' eight rows, KV head, 128 / kSplit channels), thread =
+// (row, channel quad), every kSplit-th partial.  The prefix partials' loads do
+// not wait for anything; the (max, sum) pairs of all partials meet in shared
+// memory, and every thread forms its row's weights from there.  kSplit 4 where
+// the rows alone are too few CTAs to keep some forty partials a row in flight.
 constexpr int kMaxParts = 3 * kAttnMaxCtas;
 template <int kSplit>
 __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
-    __shared__ float weight[kMaxParts][8];
-    __shared__ float red[8][8], inv_s[8];
+    constexpr int kFirst = kSplit == 1 ? 6 : 10;  // prefix partials loaded ahead
+    __shared__ float2 ml_s[kMaxParts][8];
     __shared__ float4 acc_s[kSplit == 1 ? 1 : 256];
-    pdl_wait();
-    pdl_trigger();
-    const int tid = threadIdx.x, head = blockIdx.y, r8 = tid & 7, warp = tid >> 5;
-    const uint32_t seq = blockIdx.x * 2 + r8 / kGroup;
+    __shared__ float sum_s[kSplit == 1 ? 1 : 256];
+    const int tid = threadIdx.x, head = blockIdx.y, r8 = tid & 7;
+    const uint32_t seq = min(blockIdx.x * 2 + r8 / kGroup, p.batch - 1);
     const int h = r8 % kGroup;
-    const bool there = seq < p.batch;
     // the row's partials: `n` of the prefix, `m` of its own tokens
     const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h, run = head * p.groups + mtile / 2;
     const Split prefix(p.runs * p.tiles, p.prefix_ctas);
@@ -600,88 +608,68 @@ __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_con
     const uint32_t n = (p1 - p0 + 1) * (p.dual ? 2 : 1);
     const float* base = p.prefix + ((size_t)(p0 + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
     const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
-    uint32_t m = 0, c0 = 0;
-    const float* own = nullptr;
-    if (there) {
-        const uint32_t before = p.cum[seq], units = p.cum[seq + 1] - before, all = p.cum[p.batch];
-        if (units) {
-            const uint32_t begin = before * p.heads + head * units;
-            const Split split(all * p.heads, p.own_ctas);
-            c0 = split.of(begin);
-            m = split.of(begin + units - 1) - c0 + 1;
-            own = m == 1 ? p.whole + ((size_t)seq * p.heads + head) * kPartFloats : p.part + (size_t)c0 * 2 * kPartFloats;
-        }
-    }
-    const auto own_at = [&](uint32_t i) { return own + (m == 1 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
-    // ---- weights: 32 partials at a time
-    const uint32_t total = there ? n + m : 0;
-    float l[(kMaxParts + 31) / 32], top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < (kMaxParts + 31) / 32; ++k) {
-        const uint32_t i = k * 32 + (tid >> 3);
-        if (i >= total) break;
-        const float2 ml = i < n ? __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row)
-                                : __ldcg(reinterpret_cast<const float2*>(own_at(i - n)) + h);
-        weight[i][r8] = ml.x;
-        l[k] = ml.y;
-        top = fmaxf(top, ml.x);
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    if ((tid & 31) < 8) red[warp][r8] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, red[w][r8]);
-    __syncthreads();
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < (kMaxParts + 31) / 32; ++k) {
-        const uint32_t i = k * 32 + (tid >> 3);
-        if (i >= total) break;
-        // (all -infinity: no token, sums 0; a NaN sum comes through)
-        const float f = top == -INFINITY ? 1.0f : exp2_ftz(weight[i][r8] - top);
-        weight[i][r8] = f;
-        sum = fmaf(f, l[k], sum);
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    if ((tid & 31) < 8) red[warp][r8] = sum;
-    __syncthreads();
-    if (tid < 8) {
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) s += red[w][r8];
-        inv_s[r8] = s > 0.0f ? 1.0f / s : (s == s ? 0.0f : s);
-    }
-    __syncthreads();
-    // ---- sums
     const int quad = kSplit == 1 ? tid >> 3 : blockIdx.z * (32 / kSplit) + (tid >> 3) % (32 / kSplit);
     const uint32_t part = kSplit == 1 ? 0 : (tid >> 3) / (32 / kSplit);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const auto add = [&](uint32_t i, float4 v) {
-        const float f = weight[i][r8];
-        acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
-    };
-    if (there) {
-        uint32_t i = part;
-        const float4* at = reinterpret_cast<const float4*>(base) + quad * kTileRows + row;
-#pragma unroll 8
-        for (; i < n; i += kSplit) add(i, __ldcg(at + i * step / 4));
-        for (; i < total; i += kSplit)
-            add(i, __ldcg(reinterpret_cast<const float4*>(own_at(i - n) + 2 * kGroup + h * kDim) + quad));
+    const float4* at = reinterpret_cast<const float4*>(base) + quad * kTileRows + row;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t before = p.cum[seq], after = p.cum[seq + 1], all = p.cum[p.batch];
+    float4 v[kFirst];
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) {
+        const uint32_t i = part + k * kSplit;
+        if (i < n) v[k] = __ldcg(at + i * step / 4);
     }
+    for (uint32_t i = tid >> 3; i < n; i += 32)
+        ml_s[i][r8] = __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row);
+    uint32_t m = 0;
+    const float* own = nullptr;
+    if (after > before) {
+        const uint32_t units = after - before, begin = before * p.heads + head * units;
+        const Split split(all * p.heads, p.own_ctas);
+        const uint32_t c0 = split.of(begin);
+        m = split.of(begin + units - 1) - c0 + 1;
+        own = m == 1 ? p.whole + ((size_t)seq * p.heads + head) * kPartFloats : p.part + (size_t)c0 * 2 * kPartFloats;
+    }
+    const auto own_at = [&](uint32_t i) { return own + (m == 1 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
+    for (uint32_t i = tid >> 3; i < m; i += 32) ml_s[n + i][r8] = __ldcg(reinterpret_cast<const float2*>(own_at(i)) + h);
+    __syncthreads();
+    const uint32_t total = n + m;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (uint32_t i = 0; i < total; ++i) top = fmaxf(top, ml_s[i][r8].x);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    const auto add = [&](uint32_t i, float4 x) {
+        const float2 ml = ml_s[i][r8];
+        // (all -infinity: no token, sums 0; a NaN sum comes through)
+        const float f = top == -INFINITY ? 1.0f : exp2_ftz(ml.x - top);
+        sum = fmaf(f, ml.y, sum);
+        acc = make_float4(fmaf(f, x.x, acc.x), fmaf(f, x.y, acc.y), fmaf(f, x.z, acc.z), fmaf(f, x.w, acc.w));
+    };
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) {
+        const uint32_t i = part + k * kSplit;
+        if (i < n) add(i, v[k]);
+    }
+#pragma unroll 4
+    for (uint32_t i = part + kFirst * kSplit; i < n; i += kSplit) add(i, __ldcg(at + i * step / 4));
+    for (uint32_t i = part; i < m; i += kSplit)
+        add(n + i, __ldcg(reinterpret_cast<const float4*>(own_at(i) + 2 * kGroup + h * kDim) + quad));
     if constexpr (kSplit > 1) {
         acc_s[tid] = acc;
+        sum_s[tid] = sum;
         __syncthreads();
         if (part) return;
 #pragma unroll
         for (int k = 1; k < kSplit; ++k) {
-            const float4 v = acc_s[tid + k * (256 / kSplit)];
-            acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+            const float4 x = acc_s[tid + k * (256 / kSplit)];
+            acc = make_float4(acc.x + x.x, acc.y + x.y, acc.z + x.z, acc.w + x.w);
+            sum += sum_s[tid + k * (256 / kSplit)];
         }
     }
-    if (!there) return;
-    const float inv = inv_s[r8];
+    if (blockIdx.x * 2 + r8 / kGroup >= p.batch) return;
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
     const __half2 a = __floats2half2_rn(acc.x * inv, acc.y * inv), b = __floats2half2_rn(acc.z * inv, acc.w * inv);
     reinterpret_cast<uint2*>(p.out + (((size_t)seq * p.heads + head) * kGroup + h) * kDim)[quad] =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
