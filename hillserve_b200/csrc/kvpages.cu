@@ -27,94 +27,176 @@ struct AppendParams {
     hsb_device_status* status;
 };
 
-// The last sequence whose first row is <= row; -1 for a row of none.  The
-// lanes probe 32 places at once: two rounds for 1024 sequences.
+// The last sequence whose first row is <= row; -1 for a row of none.
 __device__ __forceinline__ long long sequence_of(const int32_t* offsets, unsigned long long batch, long long row) {
-    const int lane = threadIdx.x & 31;
-    if (row >= offsets[batch]) return -1;
+    if (row >= offsets[batch] || row < offsets[0]) return -1;
     unsigned long long first = 0, n = batch;
-    while (true) {
-        const unsigned long long step = (n + 31) / 32;
-        const unsigned long long at = lane * step;
-        const unsigned under = __ballot_sync(0xffffffffu, at < n && offsets[first + at] <= row);
-        if (!under) return -1;
-        const unsigned long long skip = (31 - __clz(under)) * step;
-        first += skip;
-        n = min(step, n - skip);
-        if (step == 1) return (long long)first;
-    }
-}
-
-// A warp takes U heads of a row; half-warp 0 the K vector, half-warp 1 the V
-// vector, a lane 8 channels (one 16-byte load).
-template <int F, int U>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
-    using Fmt = PageFormat<F>;
-    pdl_wait();
-    pdl_trigger();
-    const int lane = threadIdx.x & 31, part = lane >> 4, l = lane & 15;
-    const unsigned groups = p.v.heads / U;
-    const unsigned long long item = (unsigned long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const unsigned long long row = item / groups;
-    const int h0 = (int)(item % groups) * U;
-    if (row >= p.rows) return;
-    uint4 w[U];
-    const uint16_t* src = (part ? p.x : p.k) + row * p.row_stride + l * 8;
-#pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = __ldcs(reinterpret_cast<const uint4*>(src + (h0 + u) * p.head_stride));
-    long long seq = (long long)row, first = seq;
-    if (p.offsets) {
-        seq = sequence_of(p.offsets, p.batch, (long long)row);
-        if (seq < 0) return;  // a row of no sequence
-        first = p.offsets[seq];
-    }
-    const unsigned long long pos = (unsigned long long)(uint32_t)p.starts[seq] + (unsigned long long)(row - first);
-    const long long page = page_of(p.v, seq, pos, p.status, (int)row);
-    if (page < 0) return;
-    const int r = (int)(pos % kPageTokens);
-    bool finite = true;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        unsigned char* block = p.v.data + ((size_t)page * p.v.heads + h0 + u) * Fmt::kBytes;
-        const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            finite &= ((words[i] & 0x7c00u) != 0x7c00u) && ((words[i] & 0x7c000000u) != 0x7c000000u);
-        if constexpr (!Fmt::kScaled) {
-            unsigned char* panel = block + (part * 2 + (l >> 3)) * kPanelBytes;
-            *reinterpret_cast<uint4*>(panel + r * 128 + (((l & 7) ^ (r & 7)) << 4)) = w[u];
+    while (n > 1) {
+        const unsigned long long half = n / 2;
+        if (offsets[first + half] <= row) {
+            first += half;
+            n -= half;
         } else {
-            float f[8], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
-                f[2 * i] = t.x;
-                f[2 * i + 1] = t.y;
-                // the largest finite magnitude: NaN and infinity do not set the scale
-                top = fmaxf(top, fabsf(t.x) < INFINITY ? fabsf(t.x) : 0.0f);
-                top = fmaxf(top, fabsf(t.y) < INFINITY ? fabsf(t.y) : 0.0f);
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float inv = top > 0.0f ? __fdiv_rn(Fmt::kTop, top) : 0.0f;
-            uint32_t code[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float y = __fmul_rn(f[i], inv);
-                y = y == y ? fminf(fmaxf(y, -Fmt::kTop), Fmt::kTop) : 0.0f;  // NaN: 0, infinity: the end of the range
-                uint32_t c;
-                if constexpr (F == HSB_KV_INT8) c = (uint32_t)__float2int_rn(y) & 0xffu;
-                else c = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-                code[i >> 2] |= c << (8 * (i & 3));
-            }
-            unsigned char* panel = block + part * kPanelBytes;
-            *reinterpret_cast<uint2*>(panel + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) =
-                make_uint2(code[0], code[1]);
-            if (l == 0)
-                reinterpret_cast<float*>(block + Fmt::kScaleOffset)[part * kPageTokens + r] = __fdiv_rn(top, Fmt::kTop);
+            n = half;
         }
     }
-    if (!__all_sync(0xffffffffu, finite) && lane == 0) raise_status(p.status, HSB_E_EXECUTOR_NONFINITE_KV, (int)row);
+    return (long long)first;
+}
+
+// Eight F16 values (four words) as codes; `inv` = top / max|x|.  Finite: the
+// products lie within the range up to one rounding, which the conversions end.
+template <int F>
+__device__ __forceinline__ uint2 codes_of(const uint32_t (&w)[4], float inv) {
+    uint32_t c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * i]));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * i + 1]));
+        const float y[4] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(b.x, inv), __fmul_rn(b.y, inv)};
+        if constexpr (F == HSB_KV_INT8) {
+            // adding 1.5 2^23 rounds to the nearest integer, ties to even, in the low byte
+            constexpr float kRound = 12582912.0f;
+            const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(y[0], kRound)), __float_as_uint(__fadd_rn(y[1], kRound)), 0x0040);
+            const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(y[2], kRound)), __float_as_uint(__fadd_rn(y[3], kRound)), 0x0040);
+            c[i] = __byte_perm(lo, hi, 0x5410);
+        } else {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+            c[i] = lo | (hi << 16);
+        }
+    }
+    return make_uint2(c[0], c[1]);
+}
+// The same with NaN (code 0) or infinities (the end of the range) among the values.
+template <int F>
+__device__ uint2 codes_of_nonfinite(const uint32_t (&w)[4], float inv) {
+    constexpr float kTop = PageFormat<F>::kTop;
+    uint32_t c[2] = {0, 0};
+    for (int i = 0; i < 8; ++i) {
+        const float x = half_value((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+        float y = __fmul_rn(x, inv);
+        y = y == y ? fminf(fmaxf(y, -kTop), kTop) : 0.0f;
+        uint32_t code;
+        if constexpr (F == HSB_KV_INT8) code = (uint32_t)__float2int_rn(y) & 0xffu;
+        else code = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        c[i >> 2] |= code << (8 * (i & 3));
+    }
+    return make_uint2(c[0], c[1]);
+}
+
+// A CTA takes `per` rows: one lane a row looks its page up while the first
+// rows are already being loaded.  A warp then takes U heads of a row at a
+// time: half-warp 0 the K vector, half-warp 1 the V vector, a lane 8 channels.
+// Bound by memory: 6.2 bytes move for 4 read.  Lookups by every warp for itself
+// (four dependent loads before each store) took 73 us for 32768 e4m3 rows.
+constexpr int kMostRows = 32;
+template <int F, int U>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p, const int per) {
+    using Fmt = PageFormat<F>;
+    __shared__ long long place[kMostRows];  // page x 64 + row in it; -1: nowhere
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane >> 4, l = lane & 15;
+    const int shift = 31 - __clz(p.v.heads / U), mask = (1 << shift) - 1;  // of a row's groups of heads
+    const unsigned long long row0 = (unsigned long long)blockIdx.x * per;
+    const int items = (int)min((unsigned long long)per, p.rows - row0) << shift;
+    const uint16_t* const src = (part ? p.x : p.k) + l * 8;
+    uint4 next[U];
+    const auto load = [&](int item) {
+        const uint16_t* at = src + (row0 + (item >> shift)) * p.row_stride + (item & mask) * U * p.head_stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = __ldcs(reinterpret_cast<const uint4*>(at + u * p.head_stride));
+    };
+    if (warp < items) load(warp);
+    if (threadIdx.x < per && row0 + threadIdx.x < p.rows) {
+        const long long row = (long long)(row0 + threadIdx.x);
+        long long seq = row, first = row, at = -1;
+        if (p.offsets) {
+            seq = sequence_of(p.offsets, p.batch, row);
+            if (seq >= 0) first = p.offsets[seq];
+        }
+        if (seq >= 0) {
+            const unsigned long long pos = (unsigned long long)(uint32_t)p.starts[seq] + (unsigned long long)(row - first);
+            const long long page = page_of(p.v, seq, pos, p.status, (int)row);
+            if (page >= 0) at = page * kPageTokens + (long long)(pos % kPageTokens);
+        }
+        place[threadIdx.x] = at;
+    }
+    __syncthreads();
+    for (int item = warp; item < items; item += kWarps) {
+        uint32_t w[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            w[u][0] = next[u].x;
+            w[u][1] = next[u].y;
+            w[u][2] = next[u].z;
+            w[u][3] = next[u].w;
+        }
+        if (item + kWarps < items) load(item + kWarps);
+        const long long at = place[item >> shift];
+        if (at < 0) continue;
+        const int r = (int)(at % kPageTokens), h0 = (item & mask) * U;
+        unsigned char* const block = p.v.data + ((size_t)(at / kPageTokens) * p.v.heads + h0) * Fmt::kBytes;
+        uint32_t top[U], most = 0;  // the largest magnitudes' bits (F16 orders as integers)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t m2 = __vmaxu2(__vmaxu2(w[u][0] & 0x7fff7fffu, w[u][1] & 0x7fff7fffu),
+                                         __vmaxu2(w[u][2] & 0x7fff7fffu, w[u][3] & 0x7fff7fffu));
+            top[u] = max(m2 & 0xffffu, m2 >> 16);
+            most = max(most, top[u]);
+        }
+        const bool odd = __any_sync(0xffffffffu, most >= 0x7c00u);
+        if (odd) {
+            if (lane == 0) raise_status(p.status, HSB_E_EXECUTOR_NONFINITE_KV, (int)(row0 + (item >> shift)));
+            // the largest finite magnitude: NaN and infinity do not set the scale
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                top[u] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a = w[u][i] & 0x7fffu, b = (w[u][i] >> 16) & 0x7fffu;
+                    top[u] = max(top[u], max(a < 0x7c00u ? a : 0u, b < 0x7c00u ? b : 0u));
+                }
+            }
+        }
+        if constexpr (!Fmt::kScaled) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                unsigned char* panel = block + (size_t)u * Fmt::kBytes + (part * 2 + (l >> 3)) * kPanelBytes;
+                *reinterpret_cast<uint4*>(panel + r * 128 + (((l & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+            }
+        } else {
+            // a vector's maximum over its 16 lanes; of four vectors, lanes 4 u .. 4 u + 3 of the half-warp end
+            // with vector u's, so each quotient is formed once
+            static_assert(U == 1 || U == 4, "one vector a half-warp, or four");
+            uint32_t mine;
+            if constexpr (U == 4) {
+                const bool b3 = l & 8, b2 = l & 4;
+                const uint32_t x0 = max(b3 ? top[2] : top[0], __shfl_xor_sync(0xffffffffu, b3 ? top[0] : top[2], 8));
+                const uint32_t x1 = max(b3 ? top[3] : top[1], __shfl_xor_sync(0xffffffffu, b3 ? top[1] : top[3], 8));
+                mine = max(b2 ? x1 : x0, __shfl_xor_sync(0xffffffffu, b2 ? x0 : x1, 4));
+            } else {
+                mine = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], 8));
+                mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 4));
+            }
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+            mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+            const float amax = half_value((uint16_t)mine);
+            const float inv = mine ? __fdiv_rn(Fmt::kTop, amax) : 0.0f;
+            const int owner = U == 4 ? l >> 2 : 0;
+            if ((U == 4 ? l & 3 : l) == 0)
+                reinterpret_cast<float*>(block + (size_t)owner * Fmt::kBytes + Fmt::kScaleOffset)[part * kPageTokens + r] =
+                    __fdiv_rn(amax, Fmt::kTop);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float by = __shfl_sync(0xffffffffu, inv, (lane & 16) + 4 * u);
+                const uint2 code = odd ? codes_of_nonfinite<F>(w[u], by) : codes_of<F>(w[u], by);
+                unsigned char* panel = block + (size_t)u * Fmt::kBytes + part * kPanelBytes;
+                *reinterpret_cast<uint2*>(panel + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = code;
+            }
+        }
+    }
 }
 
 // -------------------------------------------------------------------- read
@@ -194,10 +276,13 @@ constexpr unsigned long long kWideRows = 2048;
 template <int F>
 cudaError_t run_append(const AppendParams& p, cudaStream_t stream) {
     const bool wide = p.v.heads % 4 == 0 && p.rows >= kWideRows;
-    const unsigned long long items = p.rows * (p.v.heads / (wide ? 4 : 1));
-    const dim3 grid((unsigned)((items + kWarps - 1) / kWarps));
-    return wide ? launch_dependent(kv_append_kernel<F, 4>, grid, dim3(kThreads), 0, stream, false, p)
-                : launch_dependent(kv_append_kernel<F, 1>, grid, dim3(kThreads), 0, stream, false, p);
+    // as many rows a CTA as still leave eight CTAs to each SM, of the 8 warps' worth at least
+    const unsigned long long fill = p.rows / (8ull * device_info().sms);
+    const int least = std::max(1, kWarps / (p.v.heads / (wide ? 4 : 1)));
+    const int per = (int)std::min<unsigned long long>(kMostRows, std::max<unsigned long long>(least, fill));
+    const dim3 grid((unsigned)((p.rows + per - 1) / per));
+    return wide ? launch_dependent(kv_append_kernel<F, 4>, grid, dim3(kThreads), 0, stream, false, p, per)
+                : launch_dependent(kv_append_kernel<F, 1>, grid, dim3(kThreads), 0, stream, false, p, per);
 }
 template <int F>
 cudaError_t run_read(const ReadParams& p, cudaStream_t stream) {

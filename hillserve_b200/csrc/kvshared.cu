@@ -795,7 +795,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.heads = pages->kv_heads;
     c.out = d_out;
     const dim3 rows((unsigned)((batch + 1) / 2), pages->kv_heads);
-    if (rows.x * rows.y < 2u * device_info().sms)
+    if (rows.x * rows.y < 128)
         e = launch_dependent(kv_shared_combine_kernel<4>, dim3(rows.x, rows.y, 4), dim3(256), 0, s, false, c);
     else
         e = launch_dependent(kv_shared_combine_kernel<1>, rows, dim3(256), 0, s, false, c);
