@@ -67,7 +67,17 @@ struct Ring {
     static constexpr int kSlot = kPart + (Fmt::kScaled ? 2 * kTokens * 4 : 0);
     static constexpr int kSmem = 128 + kWarps * (kSlots * kSlot + kPartFloats * 4);
     static_assert(kSlots * kSlot >= kPartFloats * 4, "a piece fits in a warp's ring");
+#ifndef RC8
+#define RC8 1
+#define RC16 2
+#endif
+    // What a run costs besides its units (its query, its first rescaling, its results), in units.
+    static constexpr uint32_t kRunCost = F == HSB_KV_F16 ? RC16 : RC8;
     __host__ __device__ static constexpr uint32_t units(uint32_t tokens) { return (tokens + kTokens - 1) / kTokens; }
+    // Places of the line that a head of a sequence takes: idle ones for that cost, then its units.
+    __host__ __device__ static constexpr uint32_t places(uint32_t tokens) {
+        return tokens ? kRunCost + units(tokens) : 0;
+    }
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -125,19 +135,20 @@ __device__ __forceinline__ uint32_t tokens_of(const PagedAttention& p, uint32_t 
     }
     return n;
 }
-// A position in the line of units, up to `end`.
+// A position in the line, at a unit, up to `end`.
 template <typename R>
 struct Walker {
     uint32_t u, end;
     uint32_t seq, tokens, units;  // of the current run
-    uint32_t run;                 // its first unit
+    uint32_t run;                 // the place of its first unit
     int head;
     __device__ bool done() const { return u >= end; }
     __device__ uint32_t run_end() const { return run + units; }
     // Steps over one unit; true when that enters another run.
     __device__ bool step(const PagedAttention& p) {
         if (++u < run_end()) return false;
-        run += units;
+        run += units + R::kRunCost;
+        u = run;
         if (++head == p.v.heads && !done()) {
             head = 0;
             do {
@@ -160,19 +171,19 @@ __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, u
     const uint32_t b0 = min(batch, lane * per), b1 = min(batch, b0 + per);
     uint32_t mine = 0;
 #pragma unroll 4
-    for (uint32_t b = b0; b < b1; ++b) mine += R::units(tokens_of(p, b, scribe));
+    for (uint32_t b = b0; b < b1; ++b) mine += R::places(tokens_of(p, b, scribe));
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
-    const uint32_t total = __shfl_sync(0xffffffffu, upto, 31), before = upto - mine;  // units of one head
+    const uint32_t total = __shfl_sync(0xffffffffu, upto, 31), before = upto - mine;  // places of one head
     if (p.cum && scribe) {
         uint32_t c = before;
         for (uint32_t b = b0; b < b1; ++b) {
             p.cum[b] = c;
-            c += R::units(tokens_of(p, b, false));
+            c += R::places(tokens_of(p, b, false));
         }
         if (lane == 0) p.cum[batch] = total;
     }
@@ -187,14 +198,14 @@ __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, u
     k.end = u0 + parts.begin(warp + 1);
     if (k.done()) return k;
     const int shift = 31 - __clz(p.v.heads);  // heads is a power of two
-    const uint32_t rank = k.u >> shift;       // among the units of one head
+    const uint32_t rank = k.u >> shift;       // among the places of one head
     const bool here = rank >= before && rank < upto;
     uint32_t b = b0, n = 0, c = before;
     if (here) {
         while (true) {
             n = tokens_of(p, b, false);
-            if (rank < c + R::units(n)) break;
-            c += R::units(n);
+            if (rank < c + R::places(n)) break;
+            c += R::places(n);
             ++b;
         }
     }
@@ -203,8 +214,9 @@ __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, u
     k.tokens = __shfl_sync(0xffffffffu, n, src);
     k.units = R::units(k.tokens);
     const uint32_t base = __shfl_sync(0xffffffffu, c, src) << shift;
-    k.head = (int)((k.u - base) / k.units);
-    k.run = base + k.head * k.units;
+    k.head = (int)((k.u - base) / R::places(k.tokens));
+    k.run = base + k.head * R::places(k.tokens) + R::kRunCost;
+    k.u = max(k.u, k.run);
     return k;
 }
 
@@ -533,7 +545,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         }
         if (!alive) break;
         const bool begins = run_begin >= begin, ends = run_end <= k.end, whole = begins && ends;
-        k.u = stop - 1;  // to the next run
+        k.u = stop - 1;  // to the next run (or behind the part)
         k.step(p);
         if (!k.done()) load_query();
         // ---------------- the run's end here: all rows' sums, rounding + remainder
@@ -723,6 +735,10 @@ cudaError_t launch_format(int format, const PagedAttention& p, unsigned grid, cu
 }
 
 }  // namespace
+
+uint32_t paged_run_cost(int format) {
+    return format == HSB_KV_F16 ? Ring<HSB_KV_F16>::kRunCost : Ring<HSB_KV_INT8>::kRunCost;
+}
 
 unsigned paged_attention_grid(size_t units) {
     const unsigned sms = (unsigned)device_info().sms;

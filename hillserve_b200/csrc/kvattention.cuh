@@ -28,12 +28,12 @@ struct PagedAttention {
     float* part;                 // [CTA][2][kPartFloats]: runs cut at a stretch's begin, at its end
     float* whole;                // partial mode: [run][kPartFloats], runs of one stretch
     RunInfo* info;               // [CTA]
-    uint32_t* cum;               // partial mode: [batch + 1] units of one head before each sequence
+    uint32_t* cum;               // partial mode: [batch + 1] places of one head before each sequence
     hsb_device_status* status;
     float scale_log2;
 };
 
-// An even split of `units` over n: the first units % n stretches have one more than the others.
+// An even split of `units` (places of the line) over n: the first units % n stretches have one more than the others.
 struct Split {
     uint32_t each, more;
     __host__ __device__ Split(uint32_t units, uint32_t n) : each(units / n), more(units % n) {}
@@ -52,6 +52,8 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
+// Idle places before a run's units (kvattention.cu, Ring::kRunCost).
+uint32_t paged_run_cost(int format);
 unsigned paged_attention_grid(size_t units);
 cudaError_t launch_paged_partials(int format, const PagedAttention& p, unsigned grid, cudaStream_t stream);
 

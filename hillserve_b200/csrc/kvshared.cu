@@ -581,6 +581,7 @@ struct SharedCombine {
     const float* whole;
     const uint32_t* cum;
     unsigned own_ctas;
+    uint32_t run_cost;
     uint32_t batch;
     int heads;
     uint16_t* out;
@@ -625,10 +626,10 @@ __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_con
     uint32_t m = 0;
     const float* own = nullptr;
     if (after > before) {
-        const uint32_t units = after - before, begin = before * p.heads + head * units;
+        const uint32_t places = after - before, begin = before * p.heads + head * places + p.run_cost;
         const Split split(all * p.heads, p.own_ctas);
         const uint32_t c0 = split.of(begin);
-        m = split.of(begin + units - 1) - c0 + 1;
+        m = split.of(begin + places - p.run_cost - 1) - c0 + 1;
         own = m == 1 ? p.whole + ((size_t)seq * p.heads + head) * kPartFloats : p.part + (size_t)c0 * 2 * kPartFloats;
     }
     const auto own_at = [&](uint32_t i) { return own + (m == 1 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
@@ -791,6 +792,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.whole = a.whole;
     c.cum = a.cum;
     c.own_ctas = own;
+    c.run_cost = paged_run_cost(pages->format);
     c.batch = (uint32_t)batch;
     c.heads = pages->kv_heads;
     c.out = d_out;
