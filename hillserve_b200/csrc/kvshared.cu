@@ -541,19 +541,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             if (!ok) break;
             tc_fence_after();
             float* out = p.part + ((size_t)(blockIdx.x + run) * 2 + w) * kRowsFloats;
-            reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(m, l);
+            // (rows behind the batch are not read)
+            const bool wanted = (mtile + (kDual ? 0 : w)) * kTileSeqs + row / kGroup < p.batch;
+            if (wanted) reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(m, l);
             if (n > first) {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float o[32];
                     tmem_load32(o_at + c * 32, o);
                     tmem_wait_load();
+                    if (!wanted) continue;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         reinterpret_cast<float4*>(out)[(c * 8 + j) * kTileRows + row] =
                             make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 }
-            } else {  // no tile for this warpgroup
+            } else if (wanted) {  // no tile for this warpgroup
                 for (int c = 0; c < 32; ++c)
                     reinterpret_cast<float4*>(out)[c * kTileRows + row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
@@ -762,7 +765,9 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     p.part = reinterpret_cast<float*>(ws);
     p.status = d_status;
     p.scale_log2 = kScaleLog2;
-    const unsigned grid = std::min<unsigned>({g.runs * g.tiles, (unsigned)device_info().sms, kAttnMaxCtas});
+    // a tile for each warpgroup at least: more CTAs would only leave more partials
+    const unsigned units = g.runs * g.tiles, least = g.dual ? (units + 1) / 2 : units;
+    const unsigned grid = std::min<unsigned>({least, (unsigned)device_info().sms, kAttnMaxCtas});
     cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
 
