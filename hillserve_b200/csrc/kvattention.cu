@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     if (tid == 0) {
         RunInfo info{};
         info.run = -1;
-        p.info[blockIdx.x] = info;
+        p.info[blockIdx.x] = info;  // (a run that goes on writes its own behind the block's barrier)
     }
     if (stretch[0] >= stretch[1]) {
         if (!kFinal) pdl_wait();
@@ -548,19 +548,15 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         k.u = stop - 1;  // to the next run (or behind the part)
         k.step(p);
         if (!k.done()) load_query();
-        // ---------------- the run's end here: all rows' sums, rounding + remainder
+        // ---------------- the run's end here: all rows' sums, rounding + remainder.  Lanes t < 2
+        // keep head h0, lanes t >= 2 head h0 + 1, and give the other's parts away.
         const float os = Fmt::kScaled ? vref / kWeightUnit : 1.0f / kWeightUnit;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            L[j] += __shfl_xor_sync(0xffffffffu, L[j], 2);
-            L[j] += __shfl_xor_sync(0xffffffffu, L[j], 4);
-            L[j] += __shfl_xor_sync(0xffffffffu, L[j], 8);
-            L[j] += __shfl_xor_sync(0xffffffffu, L[j], 16);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[j][r] = (o[j][r] + __shfl_xor_sync(0xffffffffu, o[j][r], 2)) * os;
+        const int h = h0 + low;
+        const float top = low ? M[1] : M[0];
+        float sum = (low ? L[1] : L[0]) + __shfl_xor_sync(0xffffffffu, low ? L[0] : L[1], 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         // a whole run's results, or a piece in shared memory: one that goes on is the part's
         // last, so the ring has no more copies in flight and keeps it
         if (!whole && lane == 0) {
@@ -571,25 +567,21 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             c.ends = ends;
             c.there = 1;
         }
+        const bool final = kFinal && whole;
         float* slot = whole ? p.whole + (size_t)run * kPartFloats
                             : begins ? reinterpret_cast<float*>(ring) : heads_s + warp * kPartFloats;
-        if (!low) {
+        float* dst = final ? p.out + ((size_t)run * kGroup + h) * kDim : slot + 2 * kGroup + h * kDim;
+        const float by = final ? os * (sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum)) : os;
+        if (!final && g == 0) {
+            slot[2 * h] = top;
+            slot[2 * h + 1] = sum;
+        }
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const float inv = L[hh] > 0.0f ? 1.0f / L[hh] : (L[hh] == L[hh] ? 0.0f : L[hh]);
-                const bool final = kFinal && whole;
-                float* dst = final ? p.out + ((size_t)run * kGroup + h0 + hh) * kDim : slot + 2 * kGroup + (h0 + hh) * kDim;
-                if (!final && g == 0) {
-                    slot[2 * (h0 + hh)] = M[hh];
-                    slot[2 * (h0 + hh) + 1] = L[hh];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {  // MMA rows g, g + 8 of tile j: two neighbouring channels
-                    const int c = Fmt::kScaled ? g * 16 + 2 * j : (j >> 2) * 64 + g * 8 + (j & 3) * 2;
-                    *reinterpret_cast<float2*>(dst + c) =
-                        final ? make_float2(o[j][hh] * inv, o[j][hh + 2] * inv) : make_float2(o[j][hh], o[j][hh + 2]);
-                }
-            }
+        for (int j = 0; j < 8; ++j) {  // MMA rows g, g + 8 of tile j: two neighbouring channels
+            const float a = (low ? o[j][1] : o[j][0]) + __shfl_xor_sync(0xffffffffu, low ? o[j][0] : o[j][1], 2);
+            const float b = (low ? o[j][3] : o[j][2]) + __shfl_xor_sync(0xffffffffu, low ? o[j][2] : o[j][3], 2);
+            const int c = Fmt::kScaled ? g * 16 + 2 * j : (j >> 2) * 64 + g * 8 + (j & 3) * 2;
+            *reinterpret_cast<float2*>(dst + c) = make_float2(a * by, b * by);
         }
     }
     if (!alive) {  // gave up: copies in flight land before shared memory is released
@@ -597,67 +589,60 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         for (uint32_t j = it; j < fed; ++j) (void)mbar_wait(&full[j % kSlots], (j / kSlots) & 1);
     }
     __syncthreads();
-    // ================ the runs that crossed warps: pieces of one run, in order
-    const auto piece_at = [&](int w, int which) -> const float* {
-        return which ? reinterpret_cast<const float*>(ring0 + w * kSlots * R::kSlot) : heads_s + w * kPartFloats;
+    // ================ the runs that crossed warps: pieces of one run, in order, each run by one warp
+    static_assert(2 * kWarps <= 32, "a lane a piece");
+    const auto piece_at = [&](int i) -> const float* {
+        return i & 1 ? reinterpret_cast<const float*>(ring0 + (i >> 1) * kSlots * R::kSlot) : heads_s + (i >> 1) * kPartFloats;
     };
-    const auto fold_run = [&](int w0, int which, int w1) {
-        const Piece& c = pieces[w0][which];
+    const Piece* const mine = lane < 2 * kWarps ? &pieces[lane >> 1][lane & 1] : nullptr;
+    uint32_t there = __ballot_sync(0xffffffffu, mine && mine->there);
+    const uint32_t ends_mask = __ballot_sync(0xffffffffu, mine && mine->there && mine->ends);
+    for (int order = 0; there; ++order) {
+        // the next run's pieces: up to the one that ends it
+        const int first = __ffs(there) - 1;
+        uint32_t members = there;
+        // a piece that begins a run goes on; one that does not ends it or fills its warp's part
+        const uint32_t stop = (first & 1 ? there & ends_mask & ~(1u << first) : there & ends_mask);
+        if (stop) members &= (2u << (__ffs(stop) - 1)) - 1;
+        there &= ~members;
+        if (order % kWarps != warp) continue;
+        const Piece c = pieces[first >> 1][first & 1];
         const bool begins = c.first >= stretch[0], ends = c.last <= stretch[1];
-        for (int i = tid; i < kGroup * kDim / 2; i += kThreads) {
-            const int h = i >> 6, at = 2 * kGroup + i * 2;
-            float m[kWarps], top = -INFINITY, sum = 0.0f, a = 0.0f, b = 0.0f;
+        const int h = lane >> 3;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc[4];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const bool member = w == w0 || (w > w0 && w <= w1 && pieces[w][0].there);
-                m[w] = member ? piece_at(w, w == w0 && which)[2 * h] : INFINITY;
-                if (member) top = fmaxf(top, m[w]);
-            }
+        for (int j = 0; j < 4; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t left = members; left; left &= left - 1) top = fmaxf(top, piece_at(__ffs(left) - 1)[2 * h]);
+        for (uint32_t left = members; left; left &= left - 1) {
+            const float* part = piece_at(__ffs(left) - 1);
+            // (no token under a finite maximum: sum 0; a NaN sum comes through)
+            const float f = top == -INFINITY ? 1.0f : exp2_ftz(part[2 * h] - top);
+            sum = fmaf(f, part[2 * h + 1], sum);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (m[w] == INFINITY) continue;
-                const float* part = piece_at(w, w == w0 && which);
-                // (no token under a finite maximum: sum 0; a NaN sum comes through)
-                const float f = top == -INFINITY ? 1.0f : exp2_ftz(m[w] - top);
-                const float2 v = *reinterpret_cast<const float2*>(part + at);
-                sum = fmaf(f, part[2 * h + 1], sum);
-                a = fmaf(f, v.x, a);
-                b = fmaf(f, v.y, b);
-            }
-            if (kFinal && begins && ends) {
-                const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
-                *reinterpret_cast<float2*>(p.out + (size_t)c.id * kGroup * kDim + i * 2) = make_float2(a * inv, b * inv);
-            } else {
-                float* slot = begins && ends ? p.whole + (size_t)c.id * kPartFloats
-                                             : p.part + ((size_t)blockIdx.x * 2 + begins) * kPartFloats;
-                *reinterpret_cast<float2*>(slot + at) = make_float2(a, b);
-                if ((i & 63) == 0) {
-                    slot[2 * h] = top;
-                    slot[2 * h + 1] = sum;
-                }
+            for (int j = 0; j < 4; ++j) {
+                const float4 v = reinterpret_cast<const float4*>(part + 2 * kGroup + h * kDim)[(lane & 7) + 8 * j];
+                acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z), fmaf(f, v.w, acc[j].w));
             }
         }
-        if (tid == 0 && begins && !ends) {
+        const bool final = kFinal && begins && ends;
+        float* slot = begins && ends ? p.whole + (size_t)c.id * kPartFloats
+                                     : p.part + ((size_t)blockIdx.x * 2 + begins) * kPartFloats;
+        float* dst = final ? p.out + ((size_t)c.id * kGroup + h) * kDim : slot + 2 * kGroup + h * kDim;
+        const float by = final ? (sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum)) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            reinterpret_cast<float4*>(dst)[(lane & 7) + 8 * j] =
+                make_float4(acc[j].x * by, acc[j].y * by, acc[j].z * by, acc[j].w * by);
+        if (!final && (lane & 7) == 0) {
+            slot[2 * h] = top;
+            slot[2 * h + 1] = sum;
+        }
+        if (lane == 0 && begins && !ends) {
             RunInfo info{};
             info.run = (int)c.id;
             info.last = Split(units, gridDim.x).of(c.last - 1);
             p.info[blockIdx.x] = info;
-        }
-    };
-    int open = -1, which = 0, last = 0;
-    for (int i = 0; i <= 2 * kWarps; ++i) {  // the pieces in order: a run's are neighbours
-        const int w = i >> 1, second = i & 1;
-        const bool there = i < 2 * kWarps && pieces[w][second].there;
-        if (there) {
-            if (second || open < 0) {
-                open = w;
-                which = second;
-            }
-            last = w;
-        }
-        if (open >= 0 && (i == 2 * kWarps || (there && !second && pieces[w][0].ends))) {
-            fold_run(open, which, last);
-            open = -1;
         }
     }
     if (!kFinal) pdl_wait();
@@ -766,7 +751,7 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     if (!d_table || !table_width || table_width > kMaxTableEntries || !d_lengths || !batch || batch > kMaxBatch ||
         batch * table_width > kMaxTableEntries || !d_q || !d_out)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
-    if ((reinterpret_cast<uintptr_t>(d_q) & 15u) || (reinterpret_cast<uintptr_t>(d_out) & 7u) ||
+    if (((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) ||
         (reinterpret_cast<uintptr_t>(d_workspace) & 15u))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
     if (!d_workspace || workspace_bytes < hsb_kv_attention_workspace_bytes(batch, pages->kv_heads))
