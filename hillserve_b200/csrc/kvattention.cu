@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // per head, 2^e brings max |q| into [2^14, 2^15): neither half leaves F16's normal range
             const int qe = (int)((__float_as_uint(top) >> 23) & 0xffu);
-            const int e = (qe == 0 || qe == 0xff) ? 0 : max(-100, min(100, 141 - qe));
+            const int e = (qe == 0 || qe == 0xff) ? 0 : max(-113, min(100, 141 - qe));
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
@@ -751,9 +751,10 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     if (!d_table || !table_width || table_width > kMaxTableEntries || !d_lengths || !batch || batch > kMaxBatch ||
         batch * table_width > kMaxTableEntries || !d_q || !d_out)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
-    if (((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15u) ||
-        (reinterpret_cast<uintptr_t>(d_workspace) & 15u))
+    if (!aligned_to(16, d_q, d_out, static_cast<unsigned char*>(d_workspace)) || !aligned_to(4, d_table, d_lengths) ||
+        !aligned_to(8, d_status))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
+    if (d_out == d_q) return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
     if (!d_workspace || workspace_bytes < hsb_kv_attention_workspace_bytes(batch, pages->kv_heads))
         return record_error(HSB_E_WORKSPACE, "paged KV attention workspace missing or too small");
     PagedAttention p{};

@@ -337,9 +337,10 @@ int hsb_kv_append(const hsb_kv_pages* pages, const int32_t* d_table, size_t tabl
     if (!d_table || !table_width || !batch || !d_starts || !d_k || !d_v || !rows || rows > kMaxRows ||
         (!d_offsets && rows != batch))
         return record_error(HSB_E_KV_SHAPE, "paged KV append shape");
-    if (((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15u) || row_stride % 8 ||
-        head_stride % 8)
+    if (!aligned_to(16, d_k, d_v) || row_stride % 8 || head_stride % 8)
         return record_error(HSB_E_KV_SHAPE, "paged KV rows must be 16-byte aligned");
+    if (!aligned_to(4, d_table, d_starts, d_offsets) || !aligned_to(8, d_status))
+        return record_error(HSB_E_KV_SHAPE, "paged KV tables are misaligned");
     AppendParams p{};
     p.v = paged_view(*pages, d_table, table_width, table_width);
     p.starts = d_starts;
@@ -366,8 +367,9 @@ int hsb_kv_read(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_
     if (!kv_pages_valid(pages)) return record_error(HSB_E_KV_SHAPE, "paged KV pool arguments");
     if (!d_table || !table_width || !batch || !d_positions || !d_out || !max_rows || max_rows > kMaxRows)
         return record_error(HSB_E_KV_SHAPE, "paged KV read shape");
-    if (reinterpret_cast<uintptr_t>(d_out) & 15u)
-        return record_error(HSB_E_KV_SHAPE, "paged KV rows must be 16-byte aligned");
+    if (!aligned_to(16, d_out)) return record_error(HSB_E_KV_SHAPE, "paged KV rows must be 16-byte aligned");
+    if (!aligned_to(4, d_table, d_seqs, d_positions, d_count) || !aligned_to(8, d_status))
+        return record_error(HSB_E_KV_SHAPE, "paged KV tables are misaligned");
     ReadParams p{};
     p.v = paged_view(*pages, d_table, table_width, table_width);
     p.seqs = d_seqs;

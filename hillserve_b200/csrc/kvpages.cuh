@@ -82,6 +82,11 @@ __device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_
 }
 
 bool kv_pages_valid(const hsb_kv_pages* p);
+// Whether each of these addresses (null ones too) is a multiple of `by`.
+template <typename... P>
+bool aligned_to(uintptr_t by, const P*... at) {
+    return ((... | reinterpret_cast<uintptr_t>(at)) & (by - 1)) == 0;
+}
 PagedView paged_view(const hsb_kv_pages& p, const int32_t* table, size_t width, size_t pitch);
 
 }  // namespace hsb

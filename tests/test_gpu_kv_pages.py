@@ -305,6 +305,28 @@ def test_attention_bad_tables(cuda, fmt):
     assert e.value.status == 122
 
 
+@pytest.mark.parametrize("fmt", ko.FORMATS)
+def test_attention_many_sequences(cuda, fmt):
+    """More sequences than lanes, warps or CTAs, most of them empty or a token long."""
+    rng = np.random.default_rng(31)
+    lengths = np.where(rng.random(5000) < 0.4, 0, rng.integers(1, 4, 5000))
+    lengths[[17, 4999]] = 130, 200
+    cache, table, kvs = quick_fill(cuda, rng, fmt, 1, lengths)
+    q = rng.standard_normal((5000, 4, 128)).astype(np.float32)
+    want = np.stack([ko.attention(q[b], kv[:, 0], kv[:, 1]) for b, kv in enumerate(kvs)])
+    close(attend(cuda, cache, table, lengths, q), want, kvs, TOL32)
+
+
+@pytest.mark.parametrize("factor", [1e30, 2e36])
+def test_attention_huge_queries(cuda, factor):
+    """Logits far above F16's and exp's range: the largest takes all the weight."""
+    rng = np.random.default_rng(32)
+    cache, table, kvs = quick_fill(cuda, rng, "f16", 1, [100])
+    q = (rng.standard_normal((1, 4, 128)) * factor).astype(np.float32)
+    want = np.stack([ko.attention(q[0].astype(np.float64), kvs[0][:, 0], kvs[0][:, 1])])
+    close(attend(cuda, cache, table, [100], q), want, kvs, TOL32)
+
+
 def test_attention_nan_query_stays_in_its_head(cuda):
     rng = np.random.default_rng(6)
     cache, table, kvs = quick_fill(cuda, rng, "int8", 1, [100])
@@ -363,7 +385,7 @@ def test_shared_small(cuda, fmt, heads, prefix, lengths):
 
 @pytest.mark.parametrize("heads,prefix,lengths", [
     (8, 5000, [3, 500, 0, 64, 129]), (1, 40001, [9] * 32), (2, 4096, list(range(33))), (8, 1000, [7] * 64),
-    (1, 3001, [1] * 150), (4, 257, [200] * 65)])
+    (1, 3001, [1] * 150), (4, 257, [200] * 65), (8, 200, [0, 1, 2] * 500), (2, 700, [3] * 97), (8, 64, [1] * 600)])
 def test_shared_large(cuda, heads, prefix, lengths):
     got, want, whole = shared_case(cuda, prefix, "int8", heads, prefix, lengths)
     close(got, want, whole, TOL16)
@@ -387,6 +409,44 @@ def test_shared_growing_maximum(cuda):
     got = cache.attention_shared(dev(q), i32(own), i32([20, 0, 3]), pre, i32(table[0]), n)
     # |logit| reaches 256 here: 3 * 2^-24 * 256 + 12 * 2^-24 * 256 is 2.3e-4 a weight
     close(got, want, whole, TOL16 + 2 * 2.3e-4)
+    # the same for a batch of three M tiles, whose CTAs take several stretches
+    many = 70
+    table70, lengths = i32(np.zeros((many, 1))), i32(np.zeros(many))
+    got = cache.attention_shared(dev(np.tile(q, (24, 1, 1))[:many]), table70, lengths, pre, i32(table[0]), n)
+    want = [ko.attention(q[b], pk[:, 0], pk[:, 1]) for b in range(3)]
+    close(got, np.stack([want[b % 3] for b in range(many)]), [pk], TOL16 + 2 * 2.3e-4)
+
+
+def test_shared_nan_query_stays_in_its_row(cuda):
+    rng = np.random.default_rng(33)
+    cache, own, kvs = quick_fill(cuda, rng, "int8", 1, [10, 0, 5])
+    pre, table, (pkv,) = quick_fill(cuda, rng, "f16", 1, [200])
+    q = rng.standard_normal((3, 4, 128)).astype(np.float16)
+    whole = [np.concatenate([pkv, kv]) for kv in kvs]
+    want = np.stack([ko.attention(q[b], kv[:, 0], kv[:, 1]) for b, kv in enumerate(whole)])
+    q[1, 2, 100] = np.nan
+    got = cache.attention_shared(dev(q), i32(own), i32([10, 0, 5]), pre, i32(table[0]), 200).double().cpu().numpy()
+    assert np.isnan(got[1, 2]).all()
+    got[1, 2] = want[1, 2]
+    assert np.max(np.abs(got - want)) < TOL16 * np.max(np.abs(pkv[:, 1]))
+
+
+def test_shared_padded_batch_and_long_own_lengths(cuda):
+    """A padded batch (no own tokens, any query) beside one far longer own history than the prefix;
+    a length behind the table counts as none and is reported."""
+    rng = np.random.default_rng(34)
+    lengths = [9000, 0, 0, 1, 0]
+    got, want, whole = shared_case(cuda, 34, "e4m3", 2, 70, lengths)
+    close(got, want, whole, TOL16)
+    cache, own, kvs = quick_fill(cuda, rng, "f16", 2, [64, 64])
+    pre, table, (pkv,) = quick_fill(cuda, rng, "f16", 2, [65])
+    q = rng.standard_normal((2, 8, 128)).astype(np.float16)
+    got = cache.attention_shared(dev(q), i32(own), i32([65, 64]), pre, i32(table[0]), 65)
+    whole = [pkv, np.concatenate([pkv, kvs[1]])]
+    close(got, np.stack([ko.attention(q[b], kv[:, 0], kv[:, 1]) for b, kv in enumerate(whole)]), whole, TOL16)
+    with pytest.raises(cuda.InvalidArgument) as e:
+        cache.check()
+    assert e.value.status == 122
 
 
 def test_shared_bad_prefix_page(cuda):
@@ -467,6 +527,34 @@ def test_decode_steps_captured_and_eager(cuda, fmt):
     eager.check()
     replayed.check()
     assert bool((eager.data == replayed.data).all())
+
+
+def test_mirror_refuses_wrong_tensors(cuda):
+    import torch
+
+    cache = cuda.KVPages(4, kv_heads=2, format="int8")
+    half = cuda.KVPages(4, kv_heads=2, format="f16")
+    q, table, n = dev(np.zeros((3, 8, 128), np.float32)), i32(np.zeros((3, 2))), i32([0, 0, 0])
+    rows = dev(np.zeros((3, 2, 2, 128), np.float16))
+    for call in (lambda: cache.attention(q.half(), table, n), lambda: cache.attention(q[:2], table, n),
+                 lambda: cache.attention(q.cpu(), table, n), lambda: cache.attention(q, table.long(), n),
+                 lambda: cache.attention(q, table.T.contiguous().T, n), lambda: cache.attention(q, table[:, :0], n),
+                 lambda: cache.attention(q, table, n[:2]), lambda: cache.attention(q, table, n, out=q),
+                 lambda: cache.attention(q, table, n, out=torch.empty_like(q, dtype=torch.float16)),
+                 lambda: cache.append(rows[:2], table, n), lambda: cache.append(rows.float(), table, n),
+                 lambda: cache.append(rows[..., ::2], table, n), lambda: cache.append(rows, table, n, offsets=n),
+                 lambda: cache.append(rows[:0], table, n),
+                 lambda: cache.append(torch.zeros(3 * 513, dtype=torch.float16, device="cuda").view(3, 513)[:, 1:].view(3, 2, 2, 128), table, n),
+                 lambda: cache.read(n.long(), table), lambda: cache.read(n, table, seqs=n[:2]),
+                 lambda: cache.read(n, table, count=n), lambda: cache.read(n, table[0]),
+                 lambda: cache.attention_shared(q, table, n, half, i32([0]), 64),
+                 lambda: cache.attention_shared(q.half(), table, n, cache, i32([0]), 64),
+                 lambda: cache.attention_shared(q.half(), table, n, half, i32([0]), 65),
+                 lambda: cache.attention_shared(q.half(), table, n, half, i32([0]), 0)):
+        with pytest.raises(cuda.InvalidArgument):
+            call()
+    cache.append(rows[:0], table, n, offsets=i32([0, 0, 0, 0]))  # no rows at all is not an error
+    cache.check()
 
 
 def test_calls_on_two_streams_at_once(cuda):

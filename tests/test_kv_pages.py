@@ -45,7 +45,7 @@ def test_page_bytes(lib):
     assert lib.hsb_kv_page_bytes(3) == lib.hsb_kv_page_bytes(-1) == 0
 
 
-P = C.c_void_p(0x10000)
+P, O = C.c_void_p(0x10000), C.c_void_p(0x20000)
 
 
 def pool(data=0x10000, pages=4, fmt=1, heads=8):
@@ -91,22 +91,29 @@ def test_append_refusals(lib):
     for change in (dict(k=odd), dict(v=odd), dict(row=2044), dict(head=4)):
         assert call(lib, "hsb_kv_append", good, **change) == 120, change
         assert lib.hsb_last_error() == b"paged KV rows must be 16-byte aligned"
+    for change in (dict(table=C.c_void_p(0x10002)), dict(starts=C.c_void_p(0x10001)),
+                   dict(offsets=C.c_void_p(0x10002)), dict(status=C.c_void_p(0x10004))):
+        assert call(lib, "hsb_kv_append", good, **change) == 120, change
+        assert lib.hsb_last_error() == b"paged KV tables are misaligned"
 
 
 def test_read_refusals(lib):
     good = dict(pages=pool(), table=P, width=4, batch=2, seqs=None, positions=P, count=None, rows=5, out=P, status=None,
                 stream=None)
     for change in (dict(table=None), dict(width=0), dict(batch=0), dict(positions=None), dict(out=None), dict(rows=0),
-                   dict(rows=1 << 31), dict(out=C.c_void_p(0x10002))):
+                   dict(rows=1 << 31), dict(out=C.c_void_p(0x10002)), dict(seqs=C.c_void_p(0x10002)),
+                   dict(positions=C.c_void_p(0x10001)), dict(count=C.c_void_p(0x10002)), dict(status=C.c_void_p(0x10004))):
         assert call(lib, "hsb_kv_read", good, **change) == 120, change
 
 
 def test_attention_refusals(lib):
     size = lib.hsb_kv_attention_workspace_bytes(2, 8)
-    good = dict(pages=pool(), table=P, width=4, lengths=P, batch=2, q=P, out=P, ws=P, size=size, status=None, stream=None)
+    good = dict(pages=pool(), table=P, width=4, lengths=P, batch=2, q=P, out=O, ws=P, size=size, status=None, stream=None)
     for change in (dict(table=None), dict(width=0), dict(lengths=None), dict(batch=0), dict(batch=(1 << 20) + 1),
                    dict(q=None), dict(out=None), dict(width=1 << 32), dict(width=1 << 27, batch=2),
-                   dict(q=C.c_void_p(0x10002)), dict(out=C.c_void_p(0x10004)), dict(ws=C.c_void_p(0x10008))):
+                   dict(q=C.c_void_p(0x10008)), dict(out=C.c_void_p(0x20008)), dict(ws=C.c_void_p(0x10008)),
+                   dict(table=C.c_void_p(0x10002)), dict(lengths=C.c_void_p(0x10002)), dict(status=C.c_void_p(0x10004)),
+                   dict(out=P)):
         assert call(lib, "hsb_kv_attention", good, **change) == 120, change
     assert call(lib, "hsb_kv_attention", good, size=size - 1) == 3
     assert call(lib, "hsb_kv_attention", good, ws=None) == 3
@@ -114,11 +121,12 @@ def test_attention_refusals(lib):
 
 def test_shared_refusals(lib):
     size = lib.hsb_kv_attention_shared_workspace_bytes(2, 8, 64)
-    good = dict(prefix=pool(fmt=0), ptable=P, tokens=64, pages=pool(), table=P, width=4, lengths=P, batch=2, q=P, out=P,
+    good = dict(prefix=pool(fmt=0), ptable=P, tokens=64, pages=pool(), table=P, width=4, lengths=P, batch=2, q=P, out=O,
                 ws=P, size=size, status=None, stream=None)
     for change in (dict(prefix=pool(fmt=1)), dict(prefix=pool(fmt=0, heads=4)), dict(ptable=None), dict(tokens=0),
                    dict(table=None), dict(width=0), dict(lengths=None), dict(batch=0), dict(q=None), dict(out=None),
-                   dict(q=C.c_void_p(0x10008)), dict(out=C.c_void_p(0x10002)), dict(ws=C.c_void_p(0x10008))):
+                   dict(q=C.c_void_p(0x10008)), dict(out=C.c_void_p(0x20008)), dict(ws=C.c_void_p(0x10008)),
+                   dict(ptable=C.c_void_p(0x10002)), dict(batch=(1 << 20) + 1), dict(tokens=(1 << 30) + 1), dict(out=P)):
         assert call(lib, "hsb_kv_attention_shared", good, **change) == 120, change
     assert call(lib, "hsb_kv_attention_shared", good, size=size - 1) == 3
     assert call(lib, "hsb_kv_attention_shared", good, ws=None) == 3
