@@ -19,7 +19,9 @@
 // even and the odd tokens' tiles of it instead.
 //
 // The (KV head, M tiles, token tile) units are split evenly over the SMs; each
-// stretch of a run leaves F32 partials.  The sequences' own tokens go through
+// stretch of a run leaves F32 partials.  A stretch that ends one run and begins
+// the next pays for a second query tile and a second result, so long lines keep
+// idle places for that before each run.  The sequences' own tokens go through
 // the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
 #include <algorithm>
 
@@ -55,6 +57,7 @@ struct PrefixParams {
     const uint16_t* q;   // F16 [batch][4 heads][128]
     uint32_t batch, groups;  // groups: of M tiles (one or two)
     uint32_t runs;       // heads x groups
+    uint32_t run_cost;   // idle places of a run
     float* part;         // [stretch + run][2][kRowsFloats]
     hsb_device_status* status;
     float scale_log2;
@@ -163,11 +166,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // special-function unit alone (16 a clock) would take as long as the products:
 // 2^y = 2^n 2^f with n the nearest integer (adding 1.5 2^23 rounds to it) and
 // 2^f on [-0.5, 0.5] a polynomial of degree 4, fitted for the least largest
-// relative error (2.7e-6; a weight is rounded to F16 by 5e-4 next).
-#ifndef BYPOLY
-#define BYPOLY 4
-#endif
-constexpr int kByPolynomial = BYPOLY;
+// relative error (2.7e-6; a weight is rounded to F16 by 5e-4 next).  256 x 16461
+// took 98.8 us with every fourth pair, 102.2 with none.
+constexpr int kByPolynomial = 4;
 __device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
     constexpr float kRound = 12582912.0f;
     float ya, yb;
@@ -199,14 +200,23 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
     return true;
 }
 
-// A CTA's stretch of units, one segment (the part of a run) at a time.
+// A CTA's stretch of the line, one segment (its part of a run) at a time.  A run
+// takes `idle` places, then one for each tile.
 struct Segment {
-    uint32_t u, end, tiles;
+    uint32_t u, end, idle, places;
+    __device__ Segment(uint32_t begin, uint32_t stop, uint32_t cost, uint32_t tiles)
+        : u(begin), end(stop), idle(cost), places(cost + tiles) {
+        skip();
+    }
+    __device__ void skip() { u = max(u, run() * places + idle); }
     __device__ bool done() const { return u >= end; }
-    __device__ uint32_t run() const { return u / tiles; }
-    __device__ uint32_t first() const { return u % tiles; }
-    __device__ uint32_t count() const { return min(end - u, tiles - first()); }
-    __device__ void next() { u += count(); }
+    __device__ uint32_t run() const { return u / places; }
+    __device__ uint32_t first() const { return u % places - idle; }
+    __device__ uint32_t count() const { return min(end - u, places - u % places); }
+    __device__ void next() {
+        u += count();
+        skip();
+    }
 };
 
 template <bool kDual>
@@ -245,8 +255,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     const uint32_t tmem = tmem_s;  // columns: S 0, S 1, O 0, O 1 (128 each); P over the front of S
     pdl_wait();
     pdl_trigger();
-    const Split split(p.runs * p.tiles, gridDim.x);
-    Segment seg{split.begin(blockIdx.x), split.begin(blockIdx.x + 1), p.tiles};
+    const Split split(p.runs * (p.run_cost + p.tiles), gridDim.x);
+    Segment seg(split.begin(blockIdx.x), split.begin(blockIdx.x + 1), p.run_cost, p.tiles);
 
     if (warp >= kSoftmaxThreads / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -576,7 +586,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
 struct SharedCombine {
     // the prefix: partials [stretch + run][2][kRowsFloats]
     const float* prefix;
-    uint32_t tiles, groups, runs;
+    uint32_t tiles, groups, runs, prefix_cost;
     unsigned prefix_ctas;
     int dual;
     // the sequences' own tokens (kvattention.cuh)
@@ -608,8 +618,9 @@ __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_con
     const int h = r8 % kGroup;
     // the row's partials: `n` of the prefix, `m` of its own tokens
     const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h, run = head * p.groups + mtile / 2;
-    const Split prefix(p.runs * p.tiles, p.prefix_ctas);
-    const uint32_t p0 = prefix.of(run * p.tiles), p1 = prefix.of((run + 1) * p.tiles - 1);
+    const uint32_t run_places = p.prefix_cost + p.tiles;
+    const Split prefix(p.runs * run_places, p.prefix_ctas);
+    const uint32_t p0 = prefix.of(run * run_places + p.prefix_cost), p1 = prefix.of((run + 1) * run_places - 1);
     const uint32_t n = (p1 - p0 + 1) * (p.dual ? 2 : 1);
     const float* base = p.prefix + ((size_t)(p0 + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
     const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
@@ -749,7 +760,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
     if (d_out == d_q) return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
     const Geometry g = geometry(batch, pages->kv_heads, prefix_tokens);
-    if ((unsigned long long)g.runs * g.tiles > 0x7fffffffull)
+    if ((unsigned long long)g.runs * (g.tiles + 4) > 0x7fffffffull)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
     if (!d_workspace || workspace_bytes < g.total)
         return record_error(HSB_E_WORKSPACE, "paged KV attention workspace missing or too small");
@@ -770,6 +781,9 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     // a tile for each warpgroup at least: more CTAs would only leave more partials
     const unsigned units = g.runs * g.tiles, least = g.dual ? (units + 1) / 2 : units;
     const unsigned grid = std::min<unsigned>({least, (unsigned)device_info().sms, kAttnMaxCtas});
+    // idle places pay where a CTA has several times as many tiles (64 x 32768: 62 us without, 59 with;
+    // 256 x 16461: 94 and 91)
+    p.run_cost = units >= 6 * grid ? 2 : 0;
     cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
 
@@ -794,6 +808,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.groups = g.groups;
     c.runs = g.runs;
     c.prefix_ctas = grid;
+    c.prefix_cost = p.run_cost;
     c.dual = g.dual;
     c.part = a.part;
     c.whole = a.whole;
