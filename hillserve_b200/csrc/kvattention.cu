@@ -156,6 +156,19 @@ struct Walker {
 template <typename R>
 __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, uint32_t* stretch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (p.by_run) {
+        Walker<R> k{};
+        k.seq = blockIdx.x / p.v.heads;
+        k.head = (int)(blockIdx.x % p.v.heads);
+        k.tokens = tokens_of(p, k.seq, true);
+        k.units = R::units(k.tokens);
+        const Split parts(k.units, R::kWarps);
+        k.u = parts.begin(warp);
+        k.end = parts.begin(warp + 1);
+        stretch[0] = 0;
+        stretch[1] = *total_units = k.units;
+        return k;
+    }
     const bool scribe = blockIdx.x == 0 && warp == 0;
     const uint32_t batch = (uint32_t)p.batch, per = (batch + 31) / 32;
     const uint32_t b0 = min(batch, lane * per), b1 = min(batch, b0 + per);
@@ -244,13 +257,16 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     uint32_t units, stretch[2];
     Walker<R> k = find_part<R>(p, &units, stretch);
     __syncwarp();  // the barriers are ready
-    if (kFinal) {  // empty sequences: zeros
+    if (kFinal && p.by_run) {  // empty sequences: zeros
+        if (stretch[1] == 0)
+            for (int i = tid; i < kGroup * kDim; i += kThreads) p.out[(size_t)blockIdx.x * kGroup * kDim + i] = 0.0f;
+    } else if (kFinal) {
         for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
             if (tokens_of(p, b, false) == 0)
                 for (int i = tid; i < p.v.heads * kGroup * kDim; i += kThreads)
                     p.out[(size_t)b * p.v.heads * kGroup * kDim + i] = 0.0f;
     }
-    if (tid == 0) {
+    if (tid == 0 && !p.by_run) {
         RunInfo info{};
         info.run = -1;
         p.info[blockIdx.x] = info;  // (a run that goes on writes its own behind the block's barrier)
@@ -725,8 +741,20 @@ uint32_t paged_run_cost(int format) {
     return format == HSB_KV_F16 ? Ring<HSB_KV_F16>::kRunCost : Ring<HSB_KV_INT8>::kRunCost;
 }
 
-unsigned paged_attention_grid(size_t units) {
+// A CTA a run needs no scan of the lengths, no partials and no second launch, but
+// its eight warps are all that a run gets.  int8, 8 heads, by runs and split: one
+// sequence of 77 tokens 5.5 and 8.0 us, 512 8.4 and 8.9, 1000 11.0 and 9.9, 2000
+// 15.9 and 10.9; sixteen of up to 1000 11.3 and 15.3, 2000 17.5 and 20.1, 4000 27
+// and 25.
+bool paged_by_run(size_t batch, size_t table_width, int heads) {
+    const size_t runs = batch * heads, sms = device_info().sms;
+    return runs <= sms && table_width <= (2 * runs >= sms ? 32 : 12);
+}
+
+unsigned paged_attention_grid(size_t batch, size_t table_width, int heads) {
+    if (paged_by_run(batch, table_width, heads)) return (unsigned)(batch * heads);
     const unsigned sms = (unsigned)device_info().sms;
+    const size_t units = batch * table_width * heads;
     return (unsigned)std::max<size_t>(1, std::min<size_t>(units, std::min<unsigned>(sms, kAttnMaxCtas)));
 }
 
@@ -768,9 +796,10 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     p.status = d_status;
     p.scale_log2 = kScaleLog2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = paged_attention_grid(batch * table_width * pages->kv_heads);
+    p.by_run = paged_by_run(batch, table_width, pages->kv_heads);
+    const unsigned grid = paged_attention_grid(batch, table_width, pages->kv_heads);
     cudaError_t e = launch_format<float, true>(pages->format, p, grid, s);
-    if (e == cudaSuccess)
+    if (e == cudaSuccess && !p.by_run)
         e = launch_dependent(kv_combine_kernel, dim3(grid, kGroup), dim3(kDim), 0, s, false,
                              static_cast<const float*>(p.part), static_cast<const RunInfo*>(p.info), p.out);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");

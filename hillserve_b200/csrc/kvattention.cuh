@@ -28,6 +28,7 @@ struct PagedAttention {
     float* part;                 // [CTA][2][kPartFloats]: runs cut at a stretch's begin, at its end
     float* whole;                // partial mode: [run][kPartFloats], runs of one stretch
     RunInfo* info;               // [CTA]
+    int by_run;                  // CTA r has run r: nothing is cut, `part`, `info` and `cum` are not used
     uint32_t* cum;               // partial mode: [batch + 1] places of one head before each sequence
     hsb_device_status* status;
     float scale_log2;
@@ -54,7 +55,14 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 
 // Idle places before a run's units (kvattention.cu, Ring::kRunCost).
 uint32_t paged_run_cost(int format);
-unsigned paged_attention_grid(size_t units);
+// Whether a run is to be a CTA's whole work, by what the host knows of its length; and the grid.
+bool paged_by_run(size_t batch, size_t table_width, int heads);
+unsigned paged_attention_grid(size_t batch, size_t table_width, int heads);
+// The tokens of a sequence; a length behind the table's end counts as none.
+__device__ __forceinline__ uint32_t tokens_in(const int32_t* lengths, unsigned long long width, uint32_t b) {
+    const int32_t n = lengths[b];
+    return n < 0 || (unsigned long long)n > width * kPageTokens ? 0 : n;
+}
 cudaError_t launch_paged_partials(int format, const PagedAttention& p, unsigned grid, cudaStream_t stream);
 
 }  // namespace hsb

@@ -593,7 +593,9 @@ struct SharedCombine {
     const float* part;
     const float* whole;
     const uint32_t* cum;
-    unsigned own_ctas;
+    unsigned own_ctas;  // 0: every run is one CTA's
+    const int32_t* lengths;
+    unsigned long long table_width;
     uint32_t run_cost;
     uint32_t batch;
     int heads;
@@ -629,7 +631,14 @@ __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_con
     const float4* at = reinterpret_cast<const float4*>(base) + quad * kTileRows + row;
     pdl_wait();
     pdl_trigger();
-    const uint32_t before = p.cum[seq], after = p.cum[seq + 1], all = p.cum[p.batch];
+    uint32_t before = 0, after, all = 0;
+    if (p.own_ctas) {
+        before = p.cum[seq];
+        after = p.cum[seq + 1];
+        all = p.cum[p.batch];
+    } else {
+        after = tokens_in(p.lengths, p.table_width, seq);
+    }
     float4 v[kFirst];
 #pragma unroll
     for (int k = 0; k < kFirst; ++k) {
@@ -640,7 +649,10 @@ __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_con
         ml_s[i][r8] = __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row);
     uint32_t m = 0;
     const float* own = nullptr;
-    if (after > before) {
+    if (after && !p.own_ctas) {
+        m = 1;
+        own = p.whole + ((size_t)seq * p.heads + head) * kPartFloats;
+    } else if (after > before) {
         const uint32_t places = after - before, begin = before * p.heads + head * places + p.run_cost;
         const Split split(all * p.heads, p.own_ctas);
         const uint32_t c0 = split.of(begin);
@@ -798,7 +810,8 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     a.whole = reinterpret_cast<float*>(ws + g.whole);
     a.status = d_status;
     a.scale_log2 = kScaleLog2;
-    const unsigned own = paged_attention_grid(batch * table_width * pages->kv_heads);
+    a.by_run = paged_by_run(batch, table_width, pages->kv_heads);
+    const unsigned own = paged_attention_grid(batch, table_width, pages->kv_heads);
     e = launch_paged_partials(pages->format, a, own, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
 
@@ -813,7 +826,9 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.part = a.part;
     c.whole = a.whole;
     c.cum = a.cum;
-    c.own_ctas = own;
+    c.own_ctas = a.by_run ? 0 : own;
+    c.lengths = d_lengths;
+    c.table_width = table_width;
     c.run_cost = paged_run_cost(pages->format);
     c.batch = (uint32_t)batch;
     c.heads = pages->kv_heads;

@@ -305,6 +305,19 @@ def test_attention_bad_tables(cuda, fmt):
     assert e.value.status == 122
 
 
+@pytest.mark.parametrize("width", [5, 12, 13, 40])
+def test_attention_is_the_same_however_the_work_is_split(cuda, width):
+    """A wider table (of unused entries) makes the same runs whole CTAs' or stretches' work: only the
+    order of the last sums differs."""
+    rng = np.random.default_rng(35)
+    lengths = [300, 0, 64, 1]
+    cache, table, kvs = quick_fill(cuda, rng, "e4m3", 4, lengths, gap=7)
+    table = np.concatenate([table, np.full((4, width - table.shape[1]), -5, np.int32)], 1)
+    q = rng.standard_normal((4, 16, 128)).astype(np.float32)
+    want = np.stack([ko.attention(q[b], kv[:, 0], kv[:, 1]) for b, kv in enumerate(kvs)])
+    close(attend(cuda, cache, table, lengths, q), want, kvs, TOL32)
+
+
 @pytest.mark.parametrize("fmt", ko.FORMATS)
 def test_attention_many_sequences(cuda, fmt):
     """More sequences than lanes, warps or CTAs, most of them empty or a token long."""
