@@ -839,10 +839,10 @@ class KVPages:
         context, s = self._on(stream)
         with context:
             if out is None:
-                out = torch.empty(shape, dtype=torch.float32, device=self.device)
+                out = torch.empty_like(q)
             dst = self._arg(out, "out", torch.float32, shape)
             size = self._lib.hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
-            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            ws = self.data.new_empty(size)
             status = self._lib.hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size,
                                                 self._st, s)
         _raise(status)
@@ -867,10 +867,10 @@ class KVPages:
         context, s = self._on(stream)
         with context:
             if out is None:
-                out = torch.empty(shape, dtype=torch.float16, device=self.device)
+                out = torch.empty_like(q)
             dst = self._arg(out, "out", torch.float16, shape)
             size = self._lib.hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
-            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+            ws = self.data.new_empty(size)
             status = self._lib.hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_,
                                                        batch, qp, dst, ws.data_ptr(), size, self._st, s)
         _raise(status)
