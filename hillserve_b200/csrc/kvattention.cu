@@ -85,6 +85,9 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
     return d;
 }
+__device__ __forceinline__ void prefetch_l2(const void* at) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -252,7 +255,13 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     // Partial mode follows kv_prefix_kernel, which lets this grid start only once everything
     // before itself is complete, and whose results are not read here: only the end waits, so
     // that what follows finds both.
-    if (kFinal) pdl_wait();
+    if (kFinal) {
+        // lengths and tables into L2 before the wait (hints: what the preceding grid writes, it writes there too)
+        const size_t lines = (p.batch * p.v.width + 31) / 32, line = (size_t)tid * gridDim.x + blockIdx.x;
+        if (line < lines) prefetch_l2(p.v.table + line * 32);
+        if (line * 32 < p.batch) prefetch_l2(p.lengths + line * 32);
+        pdl_wait();
+    }
     pdl_trigger();
     uint32_t units, stretch[2];
     Walker<R> k = find_part<R>(p, &units, stretch);
@@ -285,8 +294,6 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         for (int ks = 0; ks < 8; ++ks)
             x4[ks] = load_q4(q + (Fmt::kScaled ? t * 32 + ks * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4));
     };
-    if (!k.done()) load_query();  // on its way while the ring is fed
-
     // ---- feeding: K (even) or V (odd) of unit feed.u into slot fed % kSlots
     Walker<R> feed = k;
     uint32_t fed = 0, ids_first = 0;
@@ -329,8 +336,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         if (part) fresh = feed.step(p);
         ++fed;
     };
+    if (!feed.done()) feed_one();
+    if (!k.done()) load_query();  // on its way while the rest of the ring is fed
 #pragma unroll 1
-    for (int i = 0; i < kSlots; ++i)
+    for (int i = 1; i < kSlots; ++i)
         if (!feed.done()) feed_one();
 
     const bool low = t >= 2;     // this lane's accumulator columns are the remainders' (and g >= 4 in B fragments)
