@@ -143,6 +143,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// The larger one; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // Two F32 values in a register pair, and the paired operations.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     uint64_t d;
@@ -162,6 +168,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 // One pair of kByPolynomial takes its powers of two from the FMA units, as the
 // special-function unit alone (16 a clock) would take as long as the products:
 // 2^y = 2^n 2^f with n the nearest integer (adding 1.5 2^23 rounds to it) and
@@ -173,7 +184,7 @@ __device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
     constexpr float kRound = 12582912.0f;
     float ya, yb;
     split_of(y2, ya, yb);
-    const uint64_t y = pair_of(fmaxf(ya, -126.0f), fmaxf(yb, -126.0f));  // (-infinity too: 2^-126 is 0 in F16)
+    const uint64_t y = pair_of(max_nan(ya, -126.0f), max_nan(yb, -126.0f));  // (-infinity too: 2^-126 is 0 in F16)
     const uint64_t t = add2(y, pair_of(kRound, kRound));
     const uint64_t f = add2(y, fma2(t, pair_of(-1.0f, -1.0f), pair_of(kRound, kRound)));
     uint64_t v = pair_of(0.0095701013f, 0.0095701013f);
@@ -181,11 +192,11 @@ __device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
     v = fma2(v, f, pair_of(0.2402474433f, 0.2402474433f));
     v = fma2(v, f, pair_of(0.6931217909f, 0.6931217909f));
     v = fma2(v, f, pair_of(0.9999992847f, 0.9999992847f));
-    float ta, tb, va, vb;
+    float ta, tb;
     split_of(t, ta, tb);
-    split_of(v, va, vb);
-    a = __uint_as_float(__float_as_uint(va) + (__float_as_uint(ta) << 23));
-    b = __uint_as_float(__float_as_uint(vb) + (__float_as_uint(tb) << 23));
+    // (a product, not a sum of exponents: NaN stays NaN)
+    split_of(mul2(v, pair_of(__uint_as_float((__float_as_uint(ta) << 23) + 0x3f800000u),
+                             __uint_as_float((__float_as_uint(tb) << 23) + 0x3f800000u))), a, b);
 }
 
 // Waits for a phase; gives up after kWaitLimitNs or once another role did.

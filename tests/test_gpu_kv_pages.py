@@ -444,6 +444,59 @@ def test_shared_nan_query_stays_in_its_row(cuda):
     assert np.max(np.abs(got - want)) < TOL16 * np.max(np.abs(pkv[:, 1]))
 
 
+@pytest.mark.parametrize("batch", [3, 40])
+def test_shared_nonfinite_keys(cuda, batch):
+    """A NaN key anywhere in the prefix is NaN in every row of its head and no other's; an infinite one is NaN
+    where its logit is +infinity and takes no weight where it is -infinity."""
+    rng = np.random.default_rng(35)
+    cache, own, _ = quick_fill(cuda, rng, "int8", 2, [0] * batch)
+    pre, table, (pkv,) = quick_fill(cuda, rng, "f16", 2, [200])
+    table = i32(table)
+    q = rng.standard_normal((batch, 8, 128)).astype(np.float16)
+    top = TOL16 * np.max(np.abs(pkv[:, 1]))
+    rows = pkv.astype(np.float16)
+    for t in list(range(9)) + [62, 63, 64, 65, 127, 128, 130, 199]:
+        for value in (np.nan, np.inf):
+            row = rows[t:t + 1].copy()
+            row[0, 0, 1, 5] = value
+            pre.append(dev(row), table, i32([t]))
+            got = cache.attention_shared(dev(q), i32(own), i32([0] * batch), pre, table[0], 200).double().cpu().numpy()
+            pre.append(dev(rows[t:t + 1].copy()), table, i32([t]))
+            for b in range(batch):
+                want = ko.attention(q[b, :4], pkv[:, 0, :1], pkv[:, 1, :1])
+                assert np.max(np.abs(got[b, :4] - want)) < top
+                gone = ko.attention(q[b, 4:], np.delete(pkv[:, 0, 1:], t, 0), np.delete(pkv[:, 1, 1:], t, 0))
+                for h in range(4):
+                    if np.isnan(value) or q[b, 4 + h, 5] > 0:
+                        assert np.isnan(got[b, 4 + h]).all(), (t, value, b, h)
+                    else:
+                        assert np.max(np.abs(got[b, 4 + h] - gone[h])) < top, (t, value, b, h)
+    pre.status.zero_()  # (the non-finite rows were reported)
+
+
+@pytest.mark.parametrize("lengths", [[77, 200, 5], [3000, 4000, 100]])
+@pytest.mark.parametrize("part", [0, 1])
+def test_attention_nan_rows_stay_in_their_sequence(cuda, part, lengths):
+    """A NaN in K or V of one token: that sequence's rows of that KV head, all NaN (K) or in that channel (V)."""
+    rng = np.random.default_rng(36)
+    cache, table, kvs = quick_fill(cuda, rng, "f16", 2, lengths)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float32)
+    want = np.stack([ko.attention(q[b], kv[:, 0], kv[:, 1]) for b, kv in enumerate(kvs)])
+    top = TOL32 * max(np.max(np.abs(kv[:, 1])) for kv in kvs)
+    for t in (0, 1, 31, 32, 63, 64, lengths[1] - 1):
+        row = kvs[1][t:t + 1].astype(np.float16)
+        bad = row.copy()
+        bad[0, part, 1, 9] = np.nan
+        cache.append(dev(bad), i32(table[1:2]), i32([t]))
+        got = cache.attention(dev(q), i32(table), i32(lengths)).double().cpu().numpy()
+        cache.append(dev(row), i32(table[1:2]), i32([t]))
+        lost = got[1, 4:] if part == 0 else got[1, 4:, 9]
+        assert np.isnan(lost).all(), t
+        lost[...] = want[1, 4:] if part == 0 else want[1, 4:, 9]
+        assert np.max(np.abs(got - want)) < top, t
+    cache.status.zero_()
+
+
 def test_shared_padded_batch_and_long_own_lengths(cuda):
     """A padded batch (no own tokens, any query) beside one far longer own history than the prefix;
     a length behind the table counts as none and is reported."""
