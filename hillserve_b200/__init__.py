@@ -822,7 +822,7 @@ class KVPages:
         context, s = self._on(stream)
         with context:
             if out is None:
-                out = torch.empty((n, 2, self.kv_heads, 128), dtype=torch.float16, device=self.device)
+                out = self.data.new_empty((n, 2, self.kv_heads, 128), dtype=torch.float16)
             dst = self._arg(out, "out", torch.float16, (n, 2, self.kv_heads, 128))
             status = self._lib.hsb_kv_read(self._ref, tp, width, batch, qp, pp, cp, n, dst, self._st, s) if n else 0
         _raise(status)

@@ -23,6 +23,16 @@
 // the next pays for a second query tile and a second result, so long lines keep
 // idle places for that before each run.  The sequences' own tokens go through
 // the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
+//
+// Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences on 32768
+// tokens 59.2 us, 256 on 16461 91 to 94, 8 on 4097 15.2.  A unit (two M tiles, 128
+// tokens) takes 1.95 us a SM, 1.3 PFLOP/s over the chip at the 1.6 GHz that the
+// products leave; with the softmax's arithmetic taken out it takes 1.9, so the
+// products and their operands are the bound: 192 KB of shared memory are read a
+// unit and 64 KB written, as many cycles (2048) as the products take at best.
+// Half-width logits, twice as many softmax warps, and weights handed over in
+// smaller parts gained nothing.  Outside that loop a call spends 13 us on the
+// queries, the first tile and the results, and the own tokens and the combine.
 #include <algorithm>
 
 #include "kvattention.cuh"
@@ -173,12 +183,15 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-// One pair of kByPolynomial takes its powers of two from the FMA units, as the
-// special-function unit alone (16 a clock) would take as long as the products:
+// With two M tiles one pair of kByPolynomial takes its powers of two from the FMA
+// units, as the special-function unit alone (16 a clock) would take as long as the
+// products:
 // 2^y = 2^n 2^f with n the nearest integer (adding 1.5 2^23 rounds to it) and
 // 2^f on [-0.5, 0.5] a polynomial of degree 4, fitted for the least largest
 // relative error (2.7e-6; a weight is rounded to F16 by 5e-4 next).  256 x 16461
-// took 98.8 us with every fourth pair, 102.2 with none.
+// takes 91.3 us with every fourth pair, 93.8 with every eighth, 93.2 with none; a
+// single M tile, where nothing runs beside a tile's softmax but the other tokens',
+// 15.6 (8 x 4097) and 15.2 with none.
 constexpr int kByPolynomial = 4;
 __device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
     constexpr float kRound = 12582912.0f;
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                         const int at = half * (kTileTokens / 2) + j;
                         const uint64_t y = fma2(pair_of(x[at], x[at + 1]), scale2, minus2);
                         float a, b;
-                        if ((j >> 1) % kByPolynomial == 0) {
+                        if (!kDual && (j >> 1) % kByPolynomial == 0) {
                             exp2_pair(y, a, b);
                         } else {
                             split_of(y, a, b);
@@ -618,7 +631,8 @@ struct SharedCombine {
 // not wait for anything; the (max, sum) pairs of all partials meet in shared
 // memory, and every thread forms its row's weights from there.  kSplit 4 where
 // the rows alone are too few CTAs to keep some forty partials a row in flight
-// (8 x 4097: 21 us a call with it, 27 without; 64 x 32768: 66 us with, 65 without).
+// (8 x 4097: 15.6 us a call with it, 17.9 without; 64 x 32768: 61.8 us with, 59.2
+// without).
 constexpr int kMaxParts = 3 * kAttnMaxCtas;
 template <int kSplit>
 __global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
@@ -804,8 +818,8 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     // a tile for each warpgroup at least: more CTAs would only leave more partials
     const unsigned units = g.runs * g.tiles, least = g.dual ? (units + 1) / 2 : units;
     const unsigned grid = std::min<unsigned>({least, (unsigned)device_info().sms, kAttnMaxCtas});
-    // idle places pay where a CTA has several times as many tiles (64 x 32768: 62 us without, 59 with;
-    // 256 x 16461: 94 and 91)
+    // idle places pay where a CTA has several times as many tiles (64 x 32768: 63.1 us without, 59.2 with;
+    // 256 x 16461: 94.6 and 92.5)
     p.run_cost = units >= 6 * grid ? 2 : 0;
     cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");

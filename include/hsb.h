@@ -647,7 +647,14 @@ int hsb_executor_decode_layer(const uint16_t* d_current, const float* d_rehearsa
  * end HSB_E_KV_POSITION, in *d_status (index = the row or sequence; d_status
  * may be NULL): nothing outside the pool or the table is touched, the row is
  * skipped (written) or zero (read), the page's tokens are left out of the
- * attention, and a sequence of such a length counts as empty. */
+ * attention, and a sequence of such a length counts as empty.
+ *
+ * Queries, outputs, rows and workspaces are 16-byte aligned, tables, lengths
+ * and positions 4-byte, d_status 8-byte; an attention's output is not its
+ * query.  Limits of the attention calls: batch 2^20, batch * table_width 2^27,
+ * prefix_tokens 2^30 (HSB_E_KV_SHAPE behind them).  A NaN in a query makes that
+ * head's row NaN; a NaN in an attended K or V row (an F16 pool keeps them) the
+ * rows of that sequence and KV head that it enters, and so may an infinity. */
 #define HSB_KV_F16 0
 #define HSB_KV_INT8 1
 #define HSB_KV_E4M3 2
