@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     using P = Plan<kDual>;
     constexpr int kStages = P::kStages;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], o_full[2], cleaned, last;
+    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], o_full[2], cleaned[kStages], last;
     __shared__ uint32_t tmem_s;
     __shared__ int live_s[kLive][2];  // tokens of a tile's two pages that count
     __shared__ volatile int dead;
@@ -259,9 +259,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
+            mbar_init(&cleaned[i], 1);
         }
         mbar_init(&q_full, kSoftmaxThreads);
-        mbar_init(&cleaned, 1);
         mbar_init(&last, 1);
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     }
                     fence_async_shared();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&cleaned);
+                    if (lane == 0) mbar_arrive(&cleaned[s]);
                 }
             };
             uint32_t number = 0;  // tiles of earlier segments
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
         } else if (warp == kMmaWarp) {
             // ================ products: one thread issues them all
             if (elect_one()) {
-                uint32_t it = 0, number = 0, segment = 0, weights[2] = {0, 0}, cleanings = 0;
+                uint32_t it = 0, number = 0, segment = 0, weights[2] = {0, 0}, cleanings = 0;  // (a bit a stage)
                 bool ok = true;
                 const uint64_t q_desc = operand(q_s, 16), k_desc = operand(ring_s, 16), v_desc = operand(ring_s, kTilePanel);
                 const auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && wait_phase(bar, parity, &dead); };
@@ -401,8 +401,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                 };
                 const auto take_v = [&](uint32_t tile_number) {
                     const uint32_t s = take();
-                    if (live_s[tile_number % kLive][0] + live_s[tile_number % kLive][1] < kTileTokens)
-                        wait(&cleaned, cleanings++ & 1);
+                    if (live_s[tile_number % kLive][0] + live_s[tile_number % kLive][1] < kTileTokens) {
+                        wait(&cleaned[s], cleanings >> s & 1);
+                        cleanings ^= 1u << s;
+                    }
                     return s;
                 };
                 const auto commit = [&](uint64_t* bar) {

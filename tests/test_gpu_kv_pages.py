@@ -532,6 +532,40 @@ def test_shared_bad_prefix_page(cuda):
     assert e.value.status == 121
 
 
+@pytest.mark.parametrize("batch", [3, 64, 100])
+@pytest.mark.parametrize("bad", [range(1, 24), range(0, 24, 2), range(0, 23), range(5, 7)])
+def test_shared_many_bad_prefix_pages(cuda, batch, bad):
+    """Tiles that are cleaned one after the other, faster than their products are issued."""
+    rng = np.random.default_rng(38)
+    heads, n = 2, 24 * 64 - 10
+    pre, table, (pkv,) = quick_fill(cuda, rng, "f16", heads, [n])
+    broken = table[0].copy()
+    broken[list(bad)] = -1
+    left = np.concatenate([pkv[i * 64:i * 64 + 64] for i in range(24) if i not in bad])
+    cache, own, _ = quick_fill(cuda, rng, "int8", heads, [0] * batch)
+    q = rng.standard_normal((batch, 4 * heads, 128)).astype(np.float16)
+    want = np.stack([ko.attention(q[b], left[:, 0], left[:, 1]) for b in range(batch)])
+    got = cache.attention_shared(dev(q), i32(own), i32([0] * batch), pre, i32(broken), n)
+    close(got, want, [left], TOL16)
+    with pytest.raises(cuda.InvalidArgument) as e:
+        cache.check()
+    assert e.value.status == 121
+
+
+@pytest.mark.parametrize("prefix", [40, 170, 300])
+def test_shared_ragged_prefix_of_many_runs(cuda, prefix):
+    """Several short runs a CTA, each with a ragged last tile."""
+    rng = np.random.default_rng(39)
+    batch, heads = 1500, 8
+    pre, table, (pkv,) = quick_fill(cuda, rng, "f16", heads, [prefix])
+    cache, own, _ = quick_fill(cuda, rng, "int8", heads, [0] * batch)
+    q = rng.standard_normal((batch, 4 * heads, 128)).astype(np.float16)
+    want = np.stack([ko.attention(q[b], pkv[:, 0], pkv[:, 1]) for b in range(0, batch, 37)])
+    got = cache.attention_shared(dev(q), i32(own), i32([0] * batch), pre, i32(table[0]), prefix)
+    cache.check()
+    close(got[::37], want, [pkv], TOL16)
+
+
 # ---------------------------------------------------------- as used together
 @pytest.mark.parametrize("fmt", ko.FORMATS)
 def test_decode_steps_captured_and_eager(cuda, fmt):
