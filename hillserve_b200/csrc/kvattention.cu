@@ -196,14 +196,6 @@ __device__ Walker<R> find_part(const PagedAttention& p, uint32_t* total_units, u
         if (lane >= o) upto += t;
     }
     const uint32_t total = __shfl_sync(0xffffffffu, upto, 31), before = upto - mine;  // places of one head
-    if (p.cum && scribe) {
-        uint32_t c = before;
-        for (uint32_t b = b0; b < b1; ++b) {
-            p.cum[b] = c;
-            c += R::places(tokens_of(p, b, false));
-        }
-        if (lane == 0) p.cum[batch] = total;
-    }
     const Split ctas(total * p.v.heads, gridDim.x);
     const uint32_t u0 = ctas.begin(blockIdx.x), u1 = ctas.begin(blockIdx.x + 1);
     const Split parts(u1 - u0, R::kWarps);
@@ -286,7 +278,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
                 for (int i = tid; i < p.v.heads * kGroup * kDim; i += kThreads)
                     p.out[(size_t)b * p.v.heads * kGroup * kDim + i] = 0.0f;
     }
-    if (tid == 0 && !p.by_run) {
+    if (kFinal && tid == 0 && !p.by_run) {
         RunInfo info{};
         info.run = -1;
         p.info[blockIdx.x] = info;  // (a run that goes on writes its own behind the block's barrier)
@@ -604,6 +596,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             c.there = 1;
         }
         const bool final = kFinal && whole;
+        if (!kFinal && whole && lane == 0) p.place[run] = 0;
         float* slot = whole ? p.whole + (size_t)run * kPartFloats
                             : begins ? reinterpret_cast<float*>(ring) : heads_s + warp * kPartFloats;
         float* dst = final ? p.out + ((size_t)run * kGroup + h) * kDim : slot + 2 * kGroup + h * kDim;
@@ -674,11 +667,12 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
             slot[2 * h] = top;
             slot[2 * h + 1] = sum;
         }
-        if (lane == 0 && begins && !ends) {
+        if (lane == 0 && begins && !(kFinal && ends)) {
             RunInfo info{};
             info.run = (int)c.id;
-            info.last = Split(units, gridDim.x).of(c.last - 1);
-            p.info[blockIdx.x] = info;
+            info.last = ends ? blockIdx.x : Split(units, gridDim.x).of(c.last - 1);
+            if (kFinal) p.info[blockIdx.x] = info;
+            else p.place[c.id] = ends ? 0 : cut_run(blockIdx.x, info.last - blockIdx.x + 1);
         }
     }
     if (!kFinal) pdl_wait();
@@ -756,10 +750,6 @@ cudaError_t launch_format(int format, const PagedAttention& p, unsigned grid, cu
 }
 
 }  // namespace
-
-uint32_t paged_run_cost(int format) {
-    return format == HSB_KV_F16 ? Ring<HSB_KV_F16>::kRunCost : Ring<HSB_KV_INT8>::kRunCost;
-}
 
 // A CTA a run needs no scan of the lengths, no partials and no second launch, but
 // its eight warps are all that a run gets.  int8, 8 heads, by runs and split: one

@@ -27,9 +27,9 @@ struct PagedAttention {
     float* out;                  // final mode: F32 [batch][4 heads][128]
     float* part;                 // [CTA][2][kPartFloats]: runs cut at a stretch's begin, at its end
     float* whole;                // partial mode: [run][kPartFloats], runs of one stretch
-    RunInfo* info;               // [CTA]
-    int by_run;                  // CTA r has run r: nothing is cut, `part`, `info` and `cum` are not used
-    uint32_t* cum;               // partial mode: [batch + 1] places of one head before each sequence
+    RunInfo* info;               // [CTA], final mode
+    int by_run;                  // CTA r has run r: nothing is cut, `part` and `info` are not used
+    uint32_t* place;             // partial mode: [run], of a run with tokens: 0 (in `whole`) or cut_run()
     hsb_device_status* status;
     float scale_log2;
 };
@@ -37,6 +37,7 @@ struct PagedAttention {
 // An even split of `units` (places of the line) over n: the first units % n stretches have one more than the others.
 struct Split {
     uint32_t each, more;
+    Split() = default;
     __host__ __device__ Split(uint32_t units, uint32_t n) : each(units / n), more(units % n) {}
     __host__ __device__ uint32_t begin(uint32_t c) const { return each * c + (c < more ? c : more); }
     // The stretch that holds unit u.
@@ -46,6 +47,9 @@ struct Split {
     }
 };
 
+// A run cut over `count` CTAs from `first` on: in the first CTA's part [1], the others' [0].
+__host__ __device__ constexpr uint32_t cut_run(uint32_t first, uint32_t count) { return first << 16 | count; }
+
 // 2^x; a result below the normal range is 0.
 __device__ __forceinline__ float exp2_ftz(float x) {
     float y;
@@ -53,8 +57,6 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
-// Idle places before a run's units (kvattention.cu, Ring::kRunCost).
-uint32_t paged_run_cost(int format);
 // Whether a run is to be a CTA's whole work, by what the host knows of its length; and the grid.
 bool paged_by_run(size_t batch, size_t table_width, int heads);
 unsigned paged_attention_grid(size_t batch, size_t table_width, int heads);

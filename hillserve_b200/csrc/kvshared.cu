@@ -25,14 +25,15 @@
 // the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
 //
 // Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences on 32768
-// tokens 59.2 us, 256 on 16461 91 to 94, 8 on 4097 15.2.  A unit (two M tiles, 128
-// tokens) takes 1.95 us a SM, 1.3 PFLOP/s over the chip at the 1.6 GHz that the
-// products leave; with the softmax's arithmetic taken out it takes 1.9, so the
-// products and their operands are the bound: 192 KB of shared memory are read a
+// tokens 55.4 us, 256 on 16461 88 to 92, 8 on 4097 14.2.  A unit (two M tiles, 128
+// tokens) takes a SM 1.76 us where the prefix stays in L2 (256 sequences), with no
+// waits for the weights 1.38, 1.8 PFLOP/s over the chip; where it comes from memory
+// (64 sequences) 1.95, its bytes alone 1.40.  192 KB of shared memory are read a
 // unit and 64 KB written, as many cycles (2048) as the products take at best.
-// Half-width logits, twice as many softmax warps, and weights handed over in
-// smaller parts gained nothing.  Outside that loop a call spends 13 us on the
-// queries, the first tile and the results, and the own tokens and the combine.
+// Half-width logits, twice as many softmax warps, weights handed over in smaller
+// parts, and a pair of SMs on one tile gained nothing.  Around that loop the prefix
+// kernel spends 11 us on the queries, the first tile and the results; the own tokens
+// add 11 and 20 us, the combine 7.
 #include <algorithm>
 
 #include "kvattention.cuh"
@@ -612,122 +613,131 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
 struct SharedCombine {
     // the prefix: partials [stretch + run][2][kRowsFloats]
     const float* prefix;
-    uint32_t tiles, groups, runs, prefix_cost;
-    unsigned prefix_ctas;
+    Split split;  // of its line
+    uint32_t groups, run_places, prefix_cost;
     int dual;
     // the sequences' own tokens (kvattention.cuh)
     const float* part;
     const float* whole;
-    const uint32_t* cum;
-    unsigned own_ctas;  // 0: every run is one CTA's
+    const uint32_t* place;
     const int32_t* lengths;
     unsigned long long table_width;
-    uint32_t run_cost;
     uint32_t batch;
     int heads;
     uint16_t* out;
 };
 
 // CTA = (two sequences' eight rows, KV head, 128 / kSplit channels), thread =
-// (row, channel quad), every kSplit-th partial.  The prefix partials' loads do
-// not wait for anything; the (max, sum) pairs of all partials meet in shared
-// memory, and every thread forms its row's weights from there.  kSplit 4 where
-// the rows alone are too few CTAs to keep some forty partials a row in flight
-// (8 x 4097: 15.6 us a call with it, 17.9 without; 64 x 32768: 61.8 us with, 59.2
-// without).
+// (row, kQuads quads of channels), every kSplit-th partial.  The (max, sum) pairs
+// of all partials meet in shared memory and become weights there, while the first
+// partials' outputs, whose loads wait for nothing, are on their way.  Bound by
+// latency where rows are few and by the threads' own work where they are many, so
+// with fewer rows there are more threads for them (8, 64, 128 and 256 sequences, 8
+// heads, us a call): kSplit 4 14.2, 58.3, -, 110; kSplit 2 15.4, 55.4, 58.5, 93;
+// one part and four quads a thread 17.7, 62.5, 60, 87.5.
 constexpr int kMaxParts = 3 * kAttnMaxCtas;
-template <int kSplit>
-__global__ void __launch_bounds__(256) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
-    constexpr int kFirst = kSplit == 1 ? 6 : 10;  // prefix partials loaded ahead
-    __shared__ float2 ml_s[kMaxParts][8];
-    __shared__ float4 acc_s[kSplit == 1 ? 1 : 256];
-    __shared__ float sum_s[kSplit == 1 ? 1 : 256];
-    const int tid = threadIdx.x, head = blockIdx.y, r8 = tid & 7;
+template <int kSplit, int kQuads, int kFirst>  // kFirst prefix partials are loaded ahead
+__global__ void __launch_bounds__(256 / kQuads) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
+    static_assert(kSplit == 1 || kQuads == 1, "one or the other");
+    constexpr int kThreads = 256 / kQuads, kLines = kThreads / 8;
+    __shared__ float2 ml_s[kMaxParts][8];            // (max, sum), then (weight, sum)
+    __shared__ float4 acc_s[kSplit == 1 ? 1 : kThreads];
+    __shared__ float sum_s[kSplit == 1 ? 1 : kThreads];
+    const int tid = threadIdx.x, head = blockIdx.y, r8 = tid & 7, line = tid >> 3;
     const uint32_t seq = min(blockIdx.x * 2 + r8 / kGroup, p.batch - 1);
     const int h = r8 % kGroup;
     // the row's partials: `n` of the prefix, `m` of its own tokens
-    const uint32_t mtile = seq / kTileSeqs, row = (seq % kTileSeqs) * kGroup + h, run = head * p.groups + mtile / 2;
-    const uint32_t run_places = p.prefix_cost + p.tiles;
-    const Split prefix(p.runs * run_places, p.prefix_ctas);
-    const uint32_t p0 = prefix.of(run * run_places + p.prefix_cost), p1 = prefix.of((run + 1) * run_places - 1);
+    const uint32_t mtile = blockIdx.x / (kTileSeqs / 2), row = (seq % kTileSeqs) * kGroup + h;
+    const uint32_t run = head * p.groups + mtile / 2, own_run = seq * p.heads + head;
+    const uint32_t p0 = p.split.of(run * p.run_places + p.prefix_cost), p1 = p.split.of((run + 1) * p.run_places - 1);
     const uint32_t n = (p1 - p0 + 1) * (p.dual ? 2 : 1);
     const float* base = p.prefix + ((size_t)(p0 + run) * 2 + (p.dual ? 0 : mtile & 1)) * kRowsFloats;
-    const size_t step = (size_t)(p.dual ? 1 : 2) * kRowsFloats;
-    const int quad = kSplit == 1 ? tid >> 3 : blockIdx.z * (32 / kSplit) + (tid >> 3) % (32 / kSplit);
-    const uint32_t part = kSplit == 1 ? 0 : (tid >> 3) / (32 / kSplit);
+    const uint32_t step = (p.dual ? 1 : 2) * kRowsFloats;
+    const int quad = kSplit == 1 ? line : blockIdx.z * (32 / kSplit) + line % (32 / kSplit);
+    const uint32_t part = kSplit == 1 ? 0 : line / (32 / kSplit);
     const float4* at = reinterpret_cast<const float4*>(base) + quad * kTileRows + row;
+    constexpr int kNext = kLines * kTileRows;  // float4s to the thread's second quad
     pdl_wait();
     pdl_trigger();
-    uint32_t before = 0, after, all = 0;
-    if (p.own_ctas) {
-        before = p.cum[seq];
-        after = p.cum[seq + 1];
-        all = p.cum[p.batch];
-    } else {
-        after = tokens_in(p.lengths, p.table_width, seq);
-    }
-    float4 v[kFirst];
+    const uint32_t tokens = tokens_in(p.lengths, p.table_width, seq), place = p.place[own_run];
+    float4 v[kFirst][kQuads];
 #pragma unroll
     for (int k = 0; k < kFirst; ++k) {
         const uint32_t i = part + k * kSplit;
-        if (i < n) v[k] = __ldcg(at + i * step / 4);
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q)
+            if (i < n) v[k][q] = __ldcg(at + (size_t)i * (step / 4) + q * kNext);
     }
-    for (uint32_t i = tid >> 3; i < n; i += 32)
-        ml_s[i][r8] = __ldcg(reinterpret_cast<const float2*>(base + i * step + kTileRows * kDim) + row);
-    uint32_t m = 0;
-    const float* own = nullptr;
-    if (after && !p.own_ctas) {
-        m = 1;
-        own = p.whole + ((size_t)seq * p.heads + head) * kPartFloats;
-    } else if (after > before) {
-        const uint32_t places = after - before, begin = before * p.heads + head * places + p.run_cost;
-        const Split split(all * p.heads, p.own_ctas);
-        const uint32_t c0 = split.of(begin);
-        m = split.of(begin + places - p.run_cost - 1) - c0 + 1;
-        own = m == 1 ? p.whole + ((size_t)seq * p.heads + head) * kPartFloats : p.part + (size_t)c0 * 2 * kPartFloats;
-    }
-    const auto own_at = [&](uint32_t i) { return own + (m == 1 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
-    for (uint32_t i = tid >> 3; i < m; i += 32) ml_s[n + i][r8] = __ldcg(reinterpret_cast<const float2*>(own_at(i)) + h);
+    for (uint32_t i = line; i < n; i += kLines)
+        ml_s[i][r8] = __ldcg(reinterpret_cast<const float2*>(base + (size_t)i * step + kTileRows * kDim) + row);
+    const uint32_t m = tokens == 0 ? 0 : place == 0 ? 1 : place & 0xffffu;
+    const float* own = place == 0 ? p.whole + (size_t)own_run * kPartFloats : p.part + (size_t)(place >> 16) * 2 * kPartFloats;
+    const auto own_at = [&](uint32_t i) { return own + (place == 0 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
+    for (uint32_t i = line; i < m; i += kLines) ml_s[n + i][r8] = __ldcg(reinterpret_cast<const float2*>(own_at(i)) + h);
     __syncthreads();
     const uint32_t total = n + m;
     float top = -INFINITY;
-#pragma unroll 4
-    for (uint32_t i = 0; i < total; ++i) top = fmaxf(top, ml_s[i][r8].x);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t i = line & 3; i < total; i += 4) top = fmaxf(top, ml_s[i][r8].x);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    __syncthreads();
+    // (all -infinity: no token, sums 0; a NaN sum comes through)
+    for (uint32_t i = line; i < total; i += kLines)
+        ml_s[i][r8].x = top == -INFINITY ? 1.0f : exp2_ftz(ml_s[i][r8].x - top);
+    __syncthreads();
+    float4 acc[kQuads];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float sum = 0.0f;
-    const auto add = [&](uint32_t i, float4 x) {
-        const float2 ml = ml_s[i][r8];
-        // (all -infinity: no token, sums 0; a NaN sum comes through)
-        const float f = top == -INFINITY ? 1.0f : exp2_ftz(ml.x - top);
-        sum = fmaf(f, ml.y, sum);
-        acc = make_float4(fmaf(f, x.x, acc.x), fmaf(f, x.y, acc.y), fmaf(f, x.z, acc.z), fmaf(f, x.w, acc.w));
+    const auto add = [&](float f, int q, float4 x) {
+        acc[q] = make_float4(fmaf(f, x.x, acc[q].x), fmaf(f, x.y, acc[q].y), fmaf(f, x.z, acc[q].z), fmaf(f, x.w, acc[q].w));
+    };
+    const auto weight = [&](uint32_t i) {
+        const float2 fl = ml_s[i][r8];
+        sum = fmaf(fl.x, fl.y, sum);
+        return fl.x;
     };
 #pragma unroll
     for (int k = 0; k < kFirst; ++k) {
         const uint32_t i = part + k * kSplit;
-        if (i < n) add(i, v[k]);
+        if (i < n) {
+            const float f = weight(i);
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) add(f, q, v[k][q]);
+        }
     }
 #pragma unroll 4
-    for (uint32_t i = part + kFirst * kSplit; i < n; i += kSplit) add(i, __ldcg(at + i * step / 4));
-    for (uint32_t i = part; i < m; i += kSplit)
-        add(n + i, __ldcg(reinterpret_cast<const float4*>(own_at(i) + 2 * kGroup + h * kDim) + quad));
+    for (uint32_t i = part + kFirst * kSplit; i < n; i += kSplit) {
+        const float f = weight(i);
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) add(f, q, __ldcg(at + (size_t)i * (step / 4) + q * kNext));
+    }
+    for (uint32_t i = part; i < m; i += kSplit) {
+        const float f = weight(n + i);
+        const float4* from = reinterpret_cast<const float4*>(own_at(i) + 2 * kGroup + h * kDim) + quad;
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) add(f, q, __ldcg(from + q * kLines));
+    }
     if constexpr (kSplit > 1) {
-        acc_s[tid] = acc;
+        acc_s[tid] = acc[0];
         sum_s[tid] = sum;
         __syncthreads();
         if (part) return;
 #pragma unroll
         for (int k = 1; k < kSplit; ++k) {
-            const float4 x = acc_s[tid + k * (256 / kSplit)];
-            acc = make_float4(acc.x + x.x, acc.y + x.y, acc.z + x.z, acc.w + x.w);
-            sum += sum_s[tid + k * (256 / kSplit)];
+            const float4 x = acc_s[tid + k * (kThreads / kSplit)];
+            acc[0] = make_float4(acc[0].x + x.x, acc[0].y + x.y, acc[0].z + x.z, acc[0].w + x.w);
+            sum += sum_s[tid + k * (kThreads / kSplit)];
         }
     }
     if (blockIdx.x * 2 + r8 / kGroup >= p.batch) return;
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
-    const __half2 a = __floats2half2_rn(acc.x * inv, acc.y * inv), b = __floats2half2_rn(acc.z * inv, acc.w * inv);
-    reinterpret_cast<uint2*>(p.out + (((size_t)seq * p.heads + head) * kGroup + h) * kDim)[quad] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        const __half2 a = __floats2half2_rn(acc[q].x * inv, acc[q].y * inv), b = __floats2half2_rn(acc[q].z * inv, acc[q].w * inv);
+        reinterpret_cast<uint2*>(p.out + ((size_t)own_run * kGroup + h) * kDim)[quad + q * kLines] =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -736,7 +746,7 @@ struct Geometry {
     uint32_t tiles, groups, runs;
     bool dual;
     size_t slots;  // of prefix partials
-    size_t cum, info, part, whole, total;
+    size_t place, part, whole, total;
 };
 Geometry geometry(size_t batch, int heads, size_t prefix_tokens) {
     Geometry g{};
@@ -746,9 +756,8 @@ Geometry geometry(size_t batch, int heads, size_t prefix_tokens) {
     g.groups = (uint32_t)((mtiles + 1) / 2);
     g.runs = (uint32_t)heads * g.groups;
     g.slots = std::min<size_t>((size_t)g.runs * g.tiles, kAttnMaxCtas) + g.runs;
-    g.cum = align256(g.slots * 2 * kRowsFloats * 4);
-    g.info = g.cum + align256((batch + 1) * 4);
-    g.part = g.info + align256(kAttnMaxCtas * sizeof(RunInfo));
+    g.place = align256(g.slots * 2 * kRowsFloats * 4);
+    g.part = g.place + align256(batch * heads * 4);
     g.whole = g.part + align256((size_t)kAttnMaxCtas * 2 * kPartFloats * 4);
     g.total = g.whole + align256(batch * heads * kPartFloats * 4);
     return g;
@@ -769,6 +778,12 @@ cudaError_t launch_prefix(const PrefixParams& p, unsigned grid, cudaStream_t str
         configured = device;
     }
     return launch_dependent(kv_prefix_kernel<kDual>, dim3(grid), dim3(kPrefixThreads), Plan<kDual>::kSmem, stream, false, p);
+}
+
+template <int kSplit, int kQuads, int kFirst>
+cudaError_t launch_combine(const SharedCombine& c, dim3 rows, cudaStream_t stream) {
+    return launch_dependent(kv_shared_combine_kernel<kSplit, kQuads, kFirst>, dim3(rows.x, rows.y, kSplit), dim3(256 / kQuads), 0,
+                            stream, false, c);
 }
 
 }  // namespace
@@ -831,8 +846,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     a.lengths = d_lengths;
     a.batch = batch;
     a.q = d_q;
-    a.cum = reinterpret_cast<uint32_t*>(ws + g.cum);
-    a.info = reinterpret_cast<RunInfo*>(ws + g.info);
+    a.place = reinterpret_cast<uint32_t*>(ws + g.place);
     a.part = reinterpret_cast<float*>(ws + g.part);
     a.whole = reinterpret_cast<float*>(ws + g.whole);
     a.status = d_status;
@@ -844,27 +858,24 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
 
     SharedCombine c{};
     c.prefix = p.part;
-    c.tiles = g.tiles;
+    c.split = Split(g.runs * (p.run_cost + g.tiles), grid);
     c.groups = g.groups;
-    c.runs = g.runs;
-    c.prefix_ctas = grid;
+    c.run_places = p.run_cost + g.tiles;
     c.prefix_cost = p.run_cost;
     c.dual = g.dual;
     c.part = a.part;
     c.whole = a.whole;
-    c.cum = a.cum;
-    c.own_ctas = a.by_run ? 0 : own;
+    c.place = a.place;
     c.lengths = d_lengths;
     c.table_width = table_width;
-    c.run_cost = paged_run_cost(pages->format);
     c.batch = (uint32_t)batch;
     c.heads = pages->kv_heads;
     c.out = d_out;
     const dim3 rows((unsigned)((batch + 1) / 2), pages->kv_heads);
-    if (rows.x * rows.y < 128)
-        e = launch_dependent(kv_shared_combine_kernel<4>, dim3(rows.x, rows.y, 4), dim3(256), 0, s, false, c);
-    else
-        e = launch_dependent(kv_shared_combine_kernel<1>, rows, dim3(256), 0, s, false, c);
+    const unsigned ctas = rows.x * rows.y;
+    e = ctas < 128 ? launch_combine<4, 1, 10>(c, rows, s)
+        : ctas < 768 ? launch_combine<2, 1, 6>(c, rows, s)
+                       : launch_combine<1, 4, 4>(c, rows, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
     record_error(HSB_OK, "");
     return HSB_OK;
