@@ -33,10 +33,10 @@
 // F32 partials that kv_combine_kernel folds in order.
 //
 // Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences of up
-// to 8192 int8 tokens 99.2 us, 5.6 TB/s; 64 x 32768 F16, two heads, 90.5 us,
-// 5.9 TB/s (a copy reaches 6.5); one sequence of 32768 int8 tokens 21.0 us, of
-// which 10.6 are its bytes and the rest the launch, the look-ups before the first
-// byte and the second launch.  Under the profiler (e4m3, 16 x 16384) the kernel
+// to 8192 int8 tokens 98.0 us, 5.6 TB/s; 64 x 32768 F16, two heads, 89.1 us,
+// 6.0 TB/s (a copy reaches 6.5); one sequence of 32768 int8 tokens 20.7 us, of
+// which 10.6 are its bytes, 3.4 kv_combine_kernel (4 to 5 of the longer calls) and
+// the rest the launch and the look-ups before the first byte.  Under the profiler (e4m3, 16 x 16384) the kernel
 // reads 554 MB, the pages' bytes once, at 5.9 TB/s; 889 instructions a warp and
 // page leave the issue slots two thirds idle.
 #include <algorithm>
@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
     // Partial mode follows kv_prefix_kernel, which lets this grid start only once everything
     // before itself is complete, and whose results are not read here: only the end waits, so
     // that what follows finds both.
+    pdl_trigger();
     if (kFinal) {
         // lengths and tables into L2 before the wait (hints: what the preceding grid writes, it writes there too)
         const size_t lines = (p.batch * p.v.width + 31) / 32, line = (size_t)tid * gridDim.x + blockIdx.x;
@@ -265,7 +266,6 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         if (line * 32 < p.batch) prefetch_l2(p.lengths + line * 32);
         pdl_wait();
     }
-    pdl_trigger();
     uint32_t units, stretch[2];
     Walker<R> k = find_part<R>(p, &units, stretch);
     __syncwarp();  // the barriers are ready
@@ -686,8 +686,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
 __global__ void __launch_bounds__(kDim) kv_combine_kernel(const float* __restrict__ part, const RunInfo* __restrict__ infos,
                                                          float* __restrict__ out) {
     constexpr int kFirst = 8;
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     const int h = blockIdx.y, d = threadIdx.x, lane = d & 31;
     const int room = (int)(gridDim.x - blockIdx.x);  // partials that there can be
     // the first partial is its CTA's [1], the others their CTAs' [0]

@@ -95,8 +95,8 @@ template <int F, int U>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p, const int per) {
     using Fmt = PageFormat<F>;
     __shared__ long long place[kMostRows];  // page x 64 + row in it; -1: nowhere
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = lane >> 4, l = lane & 15;
     const int shift = 31 - __clz(p.v.heads / U), mask = (1 << shift) - 1;  // of a row's groups of heads
     const unsigned long long row0 = (unsigned long long)blockIdx.x * per;
@@ -217,8 +217,8 @@ struct ReadParams {
 template <int F, int U>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
     using Fmt = PageFormat<F>;
-    pdl_wait();
     pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31, part = lane >> 4, l = lane & 15;
     const unsigned groups = p.v.heads / U;
     const unsigned long long item = (unsigned long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
