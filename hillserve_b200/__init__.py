@@ -838,11 +838,12 @@ class KVPages:
         np_ = self._arg(lengths, "lengths", torch.int32, (batch,))
         context, s = self._on(stream)
         with context:
+            # (first the workspace: the block that the last call gave back, whatever became of its result)
+            size = self._lib.hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
+            ws = self.data.new_empty(size)
             if out is None:
                 out = torch.empty_like(q)
             dst = self._arg(out, "out", torch.float32, shape)
-            size = self._lib.hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
-            ws = self.data.new_empty(size)
             status = self._lib.hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size,
                                                 self._st, s)
         _raise(status)
@@ -866,11 +867,11 @@ class KVPages:
             raise InvalidArgument(120, "prefix_tokens must be 1 .. 64 * len(prefix_table)")
         context, s = self._on(stream)
         with context:
+            size = self._lib.hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
+            ws = self.data.new_empty(size)  # (first, as in attention)
             if out is None:
                 out = torch.empty_like(q)
             dst = self._arg(out, "out", torch.float16, shape)
-            size = self._lib.hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
-            ws = self.data.new_empty(size)
             status = self._lib.hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_,
                                                        batch, qp, dst, ws.data_ptr(), size, self._st, s)
         _raise(status)
