@@ -744,6 +744,9 @@ class KVPages:
             raise InvalidArgument(120, "a paged KV pool is CUDA device memory")
         self.data, self.pages, self.device = data, int(data.shape[0]), data.device
         self._index, self._lib = data.get_device(), lib()
+        self._i32, self._f16, self._f32 = torch.int32, torch.float16, torch.float32
+        self._like = torch.empty_like
+        self._device_of, self._stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
         self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
         self._c = KvPages(data.data_ptr(), self.pages, self.FORMATS[format], self.kv_heads)
         self._ref, self._st = C.byref(self._c), self.status.data_ptr()
@@ -768,32 +771,30 @@ class KVPages:
         raise InvalidArgument(120, f"{name} must be {list(shape)}, contiguous; got {list(t.shape)}")
 
     def _table(self, table) -> tuple:
-        if table.dim() != 2 or table.numel() == 0:
+        shape = table.shape
+        if len(shape) != 2 or 0 in shape:
             raise InvalidArgument(120, "a page table is int32 [batch, width], not empty")
-        batch, width = table.shape
-        return self._arg(table, "table", _torch().int32, (batch, width)), width, batch
+        return self._arg(table, "table", self._i32, shape), shape[1], shape[0]
 
     def _on(self, stream):
         """A context in which new tensors belong to the stream of the call, and the stream."""
-        torch = _torch()
         if stream is None:
-            s = torch._C._cuda_getCurrentRawStream(self._index)
-            return (_HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)), s
+            s = self._stream_of(self._index)
+            return (_HERE if self._device_of() == self._index else _torch().cuda.device(self.device)), s
         if stream.device != self.device:
             raise InvalidArgument(120, f"the stream must be on the pool's device, {self.device}")
-        return torch.cuda.stream(stream), stream.cuda_stream
+        return _torch().cuda.stream(stream), stream.cuda_stream
 
     def append(self, rows, table, starts, offsets=None, stream=None) -> None:
         """Writes 16-bit float rows [n, 2 (K, V), kv_heads, 128] (any strides that
         are multiples of 8 over the first three axes).  Sequence b's are
         [offsets[b], offsets[b + 1]) (int32 [batch + 1]) at positions starts[b]
         onwards; without offsets row i is sequence i's next token."""
-        torch = _torch()
         tp, width, batch = self._table(table)
-        sp = self._arg(starts, "starts", torch.int32, (batch,))
-        op = 0 if offsets is None else self._arg(offsets, "offsets", torch.int32, (batch + 1,))
-        if rows.device != self.device or rows.dtype not in (torch.float16, torch.int16) or \
-                rows.dim() != 4 or tuple(rows.shape[1:]) != (2, self.kv_heads, 128) or rows.stride(3) != 1:
+        sp = self._arg(starts, "starts", self._i32, (batch,))
+        op = 0 if offsets is None else self._arg(offsets, "offsets", self._i32, (batch + 1,))
+        if rows.get_device() != self._index or (rows.dtype is not self._f16 and rows.dtype is not _torch().int16) or \
+                rows.shape[1:] != (2, self.kv_heads, 128) or rows.stride(3) != 1:
             raise InvalidArgument(120, f"rows must be float16 [n, 2, {self.kv_heads}, 128] on {self.device}")
         n = rows.shape[0]
         if n == 0:
@@ -813,17 +814,18 @@ class KVPages:
         """F16 rows [n, 2, kv_heads, 128] of positions (int32 [n]) of sequences
         seqs (int32 [n]; sequence 0 without them).  count (int32 [1], on the
         device): only the first count rows are written."""
-        torch = _torch()
         tp, width, batch = self._table(table)
         n = positions.numel()
-        pp = self._arg(positions, "positions", torch.int32, (n,))
-        qp = 0 if seqs is None else self._arg(seqs, "seqs", torch.int32, (n,))
-        cp = 0 if count is None else self._arg(count, "count", torch.int32, (1,))
+        pp = self._arg(positions, "positions", self._i32, (n,))
+        qp = 0 if seqs is None else self._arg(seqs, "seqs", self._i32, (n,))
+        cp = 0 if count is None else self._arg(count, "count", self._i32, (1,))
         context, s = self._on(stream)
         with context:
             if out is None:
-                out = self.data.new_empty((n, 2, self.kv_heads, 128), dtype=torch.float16)
-            dst = self._arg(out, "out", torch.float16, (n, 2, self.kv_heads, 128))
+                out = self.data.new_empty((n, 2, self.kv_heads, 128), dtype=self._f16)
+                dst = out.data_ptr()
+            else:
+                dst = self._arg(out, "out", self._f16, (n, 2, self.kv_heads, 128))
             status = self._lib.hsb_kv_read(self._ref, tp, width, batch, qp, pp, cp, n, dst, self._st, s) if n else 0
         _raise(status)
         return out
@@ -831,19 +833,20 @@ class KVPages:
     def attention(self, q, table, lengths, out=None, stream=None):
         """softmax(q . K / sqrt(128)) V over each sequence's first lengths[b]
         positions: q, out F32 [batch, 4 * kv_heads, 128]; zero for an empty one."""
-        torch = _torch()
         tp, width, batch = self._table(table)
         shape = (batch, 4 * self.kv_heads, 128)
-        qp = self._arg(q, "q", torch.float32, shape)
-        np_ = self._arg(lengths, "lengths", torch.int32, (batch,))
+        qp = self._arg(q, "q", self._f32, shape)
+        np_ = self._arg(lengths, "lengths", self._i32, (batch,))
         context, s = self._on(stream)
         with context:
             # (first the workspace: the block that the last call gave back, whatever became of its result)
             size = self._lib.hsb_kv_attention_workspace_bytes(batch, self.kv_heads)
             ws = self.data.new_empty(size)
             if out is None:
-                out = torch.empty_like(q)
-            dst = self._arg(out, "out", torch.float32, shape)
+                out = self._like(q)
+                dst = out.data_ptr()
+            else:
+                dst = self._arg(out, "out", self._f32, shape)
             status = self._lib.hsb_kv_attention(self._ref, tp, width, np_, batch, qp, dst, ws.data_ptr(), size,
                                                 self._st, s)
         _raise(status)
@@ -854,12 +857,11 @@ class KVPages:
         """attention for a batch whose sequences share their first
         prefix_tokens positions, kept in an F16 pool and read once for all;
         table and lengths are of each sequence's own tokens.  q, out F16."""
-        torch = _torch()
         tp, width, batch = self._table(table)
         shape = (batch, 4 * self.kv_heads, 128)
-        qp = self._arg(q, "q", torch.float16, shape)
-        np_ = self._arg(lengths, "lengths", torch.int32, (batch,))
-        ptp = self._arg(prefix_table, "prefix_table", torch.int32, (prefix_table.numel(),))
+        qp = self._arg(q, "q", self._f16, shape)
+        np_ = self._arg(lengths, "lengths", self._i32, (batch,))
+        ptp = self._arg(prefix_table, "prefix_table", self._i32, (prefix_table.numel(),))
         prefix_tokens = int(prefix_tokens)
         if prefix.device != self.device:
             raise InvalidArgument(120, "the prefix must be on the pool's device")
@@ -870,8 +872,10 @@ class KVPages:
             size = self._lib.hsb_kv_attention_shared_workspace_bytes(batch, self.kv_heads, prefix_tokens)
             ws = self.data.new_empty(size)  # (first, as in attention)
             if out is None:
-                out = torch.empty_like(q)
-            dst = self._arg(out, "out", torch.float16, shape)
+                out = self._like(q)
+                dst = out.data_ptr()
+            else:
+                dst = self._arg(out, "out", self._f16, shape)
             status = self._lib.hsb_kv_attention_shared(prefix._ref, ptp, prefix_tokens, self._ref, tp, width, np_,
                                                        batch, qp, dst, ws.data_ptr(), size, self._st, s)
         _raise(status)

@@ -124,12 +124,6 @@ __device__ __forceinline__ float4 load_q4(const uint16_t* q) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// True in one lane of the warp.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t one;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-    return one != 0;
-}
 // Tokens of a sequence; a length behind the table's end counts as none.
 __device__ __forceinline__ uint32_t tokens_of(const PagedAttention& p, uint32_t b, bool report) {
     const int32_t n = p.lengths[b];
@@ -651,7 +645,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float4 v = reinterpret_cast<const float4*>(part + 2 * kGroup + h * kDim)[(lane & 7) + 8 * j];
-                acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z), fmaf(f, v.w, acc[j].w));
+                acc[j] = make_float4(fmaf(f, v.x, acc[j].x), fmaf(f, v.y, acc[j].y), fmaf(f, v.z, acc[j].z),
+                                     fmaf(f, v.w, acc[j].w));
             }
         }
         const bool final = kFinal && begins && ends;
@@ -725,8 +720,6 @@ __global__ void __launch_bounds__(kDim) kv_combine_kernel(const float* __restric
     out[((size_t)info.run * kGroup + h) * kDim + d] = acc * (L > 0.0f ? 1.0f / L : (L == L ? 0.0f : L));
 }
 
-size_t align256(size_t b) { return (b + 255) / 256 * 256; }
-
 template <int F, typename Q, bool kFinal>
 cudaError_t launch(const PagedAttention& p, unsigned grid, cudaStream_t stream) {
     static thread_local int configured = -1;
@@ -737,7 +730,8 @@ cudaError_t launch(const PagedAttention& p, unsigned grid, cudaStream_t stream) 
         if (e != cudaSuccess) return e;
         configured = device;
     }
-    return launch_dependent(kv_attention_kernel<F, Q, kFinal>, dim3(grid), dim3(Ring<F>::kThreads), Ring<F>::kSmem, stream, false, p);
+    return launch_dependent(kv_attention_kernel<F, Q, kFinal>, dim3(grid), dim3(Ring<F>::kThreads), Ring<F>::kSmem, stream,
+                            false, p);
 }
 
 template <typename Q, bool kFinal>

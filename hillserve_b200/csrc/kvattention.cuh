@@ -57,6 +57,14 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
+inline size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
 // Whether a run is to be a CTA's whole work, by what the host knows of its length; and the grid.
 bool paged_by_run(size_t batch, size_t table_width, int heads);
 unsigned paged_attention_grid(size_t batch, size_t table_width, int heads);

@@ -56,9 +56,10 @@ __device__ __forceinline__ uint2 codes_of(const uint32_t (&w)[4], float inv) {
         if constexpr (F == HSB_KV_INT8) {
             // adding 1.5 2^23 rounds to the nearest integer, ties to even, in the low byte
             constexpr float kRound = 12582912.0f;
-            const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(y[0], kRound)), __float_as_uint(__fadd_rn(y[1], kRound)), 0x0040);
-            const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(y[2], kRound)), __float_as_uint(__fadd_rn(y[3], kRound)), 0x0040);
-            c[i] = __byte_perm(lo, hi, 0x5410);
+            uint32_t r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = __float_as_uint(__fadd_rn(y[j], kRound));
+            c[i] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
         } else {
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);

@@ -25,7 +25,7 @@
 // the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
 //
 // Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences on 32768
-// tokens 55.4 us, 256 on 16461 88 to 92, 8 on 4097 14.2.  A unit (two M tiles, 128
+// tokens 55.4 us, 256 on 16461 88 to 94, 8 on 4097 14.2.  A unit (two M tiles, 128
 // tokens) takes a SM 1.76 us where the prefix stays in L2 (256 sequences), with no
 // waits for the weights 1.38, 1.8 PFLOP/s over the chip; where it comes from memory
 // (64 sequences) 1.95, its bytes alone 1.40.  192 KB of shared memory are read a
@@ -139,12 +139,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// True in one lane of the warp.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t one;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-    return one != 0;
-}
 // Generic writes to shared memory before the tensor cores or bulk copies use it.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -308,7 +302,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             };
             const auto load = [&](uint32_t tile, int head, int part, uint32_t number) {
                 const uint32_t s = it % kStages;
-                if (it >= (uint32_t)kStages) ok = ok && __all_sync(0xffffffffu, wait_phase(&empty[s], ((it / kStages) - 1) & 1, &dead));
+                if (it >= (uint32_t)kStages)
+                    ok = ok && __all_sync(0xffffffffu, wait_phase(&empty[s], ((it / kStages) - 1) & 1, &dead));
                 if (!ok) return;
                 const int from = (int)(tile - ids_first) * 2 + (lane & 1);
                 const int32_t id = __shfl_sync(0xffffffffu, id32, from);
@@ -521,7 +516,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                 for (int j = 4; j < kTileTokens; j += 8) {
 #pragma unroll
                     for (int i4 = 0; i4 < 4; ++i4)
-                        tops[i4] = j + 4 + i4 < kTileTokens ? max3(tops[i4], x[j + i4], x[j + 4 + i4]) : fmaxf(tops[i4], x[j + i4]);
+                        tops[i4] = j + 4 + i4 < kTileTokens ? max3(tops[i4], x[j + i4], x[j + 4 + i4])
+                                                            : fmaxf(tops[i4], x[j + i4]);
                 }
                 float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
                 top *= p.scale_log2;
@@ -734,13 +730,12 @@ __global__ void __launch_bounds__(256 / kQuads) kv_shared_combine_kernel(const _
     const float inv = sum > 0.0f ? 1.0f / sum : (sum == sum ? 0.0f : sum);
 #pragma unroll
     for (int q = 0; q < kQuads; ++q) {
-        const __half2 a = __floats2half2_rn(acc[q].x * inv, acc[q].y * inv), b = __floats2half2_rn(acc[q].z * inv, acc[q].w * inv);
+        const __half2 a = __floats2half2_rn(acc[q].x * inv, acc[q].y * inv);
+        const __half2 b = __floats2half2_rn(acc[q].z * inv, acc[q].w * inv);
         reinterpret_cast<uint2*>(p.out + ((size_t)own_run * kGroup + h) * kDim)[quad + q * kLines] =
             make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
 }
-
-size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 struct Geometry {
     uint32_t tiles, groups, runs;
