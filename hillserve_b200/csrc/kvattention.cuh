@@ -49,6 +49,11 @@ struct Split {
 
 // A run cut over `count` CTAs from `first` on: in the first CTA's part [1], the others' [0].
 __host__ __device__ constexpr uint32_t cut_run(uint32_t first, uint32_t count) { return first << 16 | count; }
+// The partials of a run with tokens, whose place is this word, in a grid of that many CTAs.  A warp that gave up
+// its wait leaves its runs' places as the workspace was: a word that names CTAs outside the grid counts as none.
+__host__ __device__ constexpr uint32_t run_partials(uint32_t place, uint32_t grid) {
+    return place == 0 ? 1 : (place >> 16) + (place & 0xffffu) <= grid ? place & 0xffffu : 0;
+}
 
 // 2^x; a result below the normal range is 0.
 __device__ __forceinline__ float exp2_ftz(float x) {

@@ -616,6 +616,7 @@ struct SharedCombine {
     const float* part;
     const float* whole;
     const uint32_t* place;
+    uint32_t own_grid;  // of the kernel that left them
     const int32_t* lengths;
     unsigned long long table_width;
     uint32_t batch;
@@ -631,7 +632,7 @@ struct SharedCombine {
 // with fewer rows there are more threads for them (8, 64, 128 and 256 sequences, 8
 // heads, us a call): kSplit 4 14.2, 58.3, -, 110; kSplit 2 15.4, 55.4, 58.5, 93;
 // one part and four quads a thread 17.7, 62.5, 60, 87.5.
-constexpr int kMaxParts = 3 * kAttnMaxCtas;
+constexpr int kMaxParts = 3 * kAttnMaxCtas;  // two a CTA of the prefix, one a CTA of the own tokens
 template <int kSplit, int kQuads, int kFirst>  // kFirst prefix partials are loaded ahead
 __global__ void __launch_bounds__(256 / kQuads) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
     static_assert(kSplit == 1 || kQuads == 1, "one or the other");
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(256 / kQuads) kv_shared_combine_kernel(const _
     }
     for (uint32_t i = line; i < n; i += kLines)
         ml_s[i][r8] = __ldcg(reinterpret_cast<const float2*>(base + (size_t)i * step + kTileRows * kDim) + row);
-    const uint32_t m = tokens == 0 ? 0 : place == 0 ? 1 : place & 0xffffu;
+    const uint32_t m = tokens == 0 ? 0 : run_partials(place, p.own_grid);
     const float* own = place == 0 ? p.whole + (size_t)own_run * kPartFloats : p.part + (size_t)(place >> 16) * 2 * kPartFloats;
     const auto own_at = [&](uint32_t i) { return own + (place == 0 ? 0 : ((size_t)i * 2 + (i == 0)) * kPartFloats); };
     for (uint32_t i = line; i < m; i += kLines) ml_s[n + i][r8] = __ldcg(reinterpret_cast<const float2*>(own_at(i)) + h);
@@ -861,6 +862,7 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     c.part = a.part;
     c.whole = a.whole;
     c.place = a.place;
+    c.own_grid = own;
     c.lengths = d_lengths;
     c.table_width = table_width;
     c.batch = (uint32_t)batch;
