@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
     using P = Plan<kDual>;
     constexpr int kStages = P::kStages;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], o_full[2], cleaned[kStages], last;
+    __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full[2], p_full[2][2], p_read[2], o_full[2], cleaned[kStages], last;
     __shared__ uint32_t tmem_s;
     __shared__ int live_s[kLive][2];  // tokens of a tile's two pages that count
     __shared__ volatile int dead;
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             mbar_init(&s_full[w], 1);
             mbar_init(&p_full[w][0], 128);
             mbar_init(&p_full[w][1], 128);
+            mbar_init(&p_read[w], 1);
             mbar_init(&o_full[w], 1);
         }
         mbar_fence_init();
@@ -371,8 +372,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     ++it;
                     return s;
                 };
-                const auto logits = [&](int w, uint32_t s) {
+                // Of a run's first tiles; later ones lie over the weights of the tile before, which that
+                // tile's product has then read (the order of two products of one thread is only given where
+                // they have the accumulator in common).
+                uint32_t weights_read[2] = {0, 0};
+                const auto logits = [&](int w, uint32_t s, bool over) {
+                    if (over) wait(&p_read[w], weights_read[w]++ & 1);
                     if (!ok) return;
+                    tc_fence_after();
                     const uint64_t a = q_desc + (kDual ? 0 : w * (kTileBytes >> 4)), b = k_desc + s * (kTileBytes >> 4);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     }
                     tc_commit(&s_full[w]);
                 };
-                const auto output = [&](int w, uint32_t s, bool add) {
+                const auto output = [&](int w, uint32_t s, bool add, bool more) {
                     const uint64_t b = v_desc + s * (kTileBytes >> 4);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // the first 64 tokens' while the others' weights are made
@@ -394,6 +401,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                                         add || k > 0);
                     }
                     ++weights[w];
+                    if (more) tc_commit(&p_read[w]);
                 };
                 const auto take_v = [&](uint32_t tile_number) {
                     const uint32_t s = take();
@@ -413,17 +421,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     if constexpr (kDual) {
                         for (uint32_t i = 0; i < 2 && i < n; ++i) {
                             const uint32_t s = take();
-                            logits(i, s);
+                            logits(i, s, false);
                             commit(&empty[s]);
                         }
                         for (uint32_t i = 0; ok && i < n; ++i) {
                             const int w = i & 1;
                             const uint32_t s = take_v(number + i);
-                            output(w, s, i >= 2);
+                            output(w, s, i >= 2, i + 2 < n);
                             commit(&empty[s]);
                             if (i + 2 < n) {
                                 const uint32_t next = take();
-                                logits(w, next);
+                                logits(w, next, true);
                                 commit(&empty[next]);
                             } else {
                                 commit(&o_full[w]);
@@ -432,22 +440,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                         if (n == 1) commit(&o_full[1]);
                     } else {
                         uint32_t s = take();
-                        logits(0, s);
-                        logits(1, s);
+                        logits(0, s, false);
+                        logits(1, s, false);
                         commit(&empty[s]);
                         for (uint32_t i = 0; ok && i < n; ++i) {
                             const uint32_t v = take_v(number + i);
-                            output(0, v, i > 0);
+                            output(0, v, i > 0, i + 1 < n);
                             if (i + 1 < n) {
                                 s = take();
-                                logits(0, s);
+                                logits(0, s, true);
                             } else {
                                 commit(&o_full[0]);
                             }
-                            output(1, v, i > 0);
+                            output(1, v, i > 0, i + 1 < n);
                             commit(&empty[v]);
                             if (i + 1 < n) {
-                                logits(1, s);
+                                logits(1, s, true);
                                 commit(&empty[s]);
                             } else {
                                 commit(&o_full[1]);
