@@ -50,6 +50,10 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9;          // of a third warpgroup, whi
 constexpr int kPrefixThreads = 384;                 // to the other two (setmaxnreg)
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 constexpr float kSlack = 8.0f;                      // weights are at most 2^8 (F16 holds 2^15)
+// Weights are 2^(logit x scale - reference), one FMA.  The reference is the largest logit's product, rounded: by 2^-4
+// at most up to 2^20, where weights may just as well be relative to it.  Behind that the rounding would leave F16's
+// range, so the difference is formed before the scale.
+constexpr float kFar = 1048576.0f;
 constexpr int kLive = 16;                           // ring of tiles' live counts
 // a partial: outputs [32 channel quads][128 rows][4], then (max, sum) [128 rows]
 constexpr int kRowsFloats = kTileRows * kDim + 2 * kTileRows;
@@ -503,7 +507,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             }
             fence_async_shared();
             mbar_arrive(&q_full);
-            float m = -INFINITY, l = 0.0f;  // the reference in log2 units; the sum
+            // The largest logit that moved the reference, before its scale; whether any of the warp's is far; the sum.
+            float most = -INFINITY, l = 0.0f;
+            bool far = false;
+            const auto reference = [&]() { return __fmul_rn(most, p.scale_log2); };  // (rounded, never part of an FMA)
+            const auto residual = [&]() { return fmaf(most, p.scale_log2, -reference()); };
             const uint32_t step = kDual ? 2 : 1, first = kDual ? w : 0;
             for (uint32_t i = first; ok && i < n; i += step) {
                 ok = __all_sync(0xffffffffu, wait_phase(&s_full[w], logits_seen++ & 1, &dead));
@@ -527,13 +535,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                         tops[i4] = j + 4 + i4 < kTileTokens ? max3(tops[i4], x[j + i4], x[j + 4 + i4])
                                                             : fmaxf(tops[i4], x[j + i4]);
                 }
-                float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-                top *= p.scale_log2;
-                if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                    const float to = fmaxf(m, top);
-                    const float f = m == -INFINITY ? 0.0f : exp2_ftz(m - to);
+                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+                if (__any_sync(0xffffffffu, (top - most) * p.scale_log2 > kSlack)) {
+                    const float to = fmaxf(most, top), before = reference();
+                    const float rest = far ? residual() : 0.0f;
+                    const bool none = most == -INFINITY;
+                    most = to;
+                    far = __any_sync(0xffffffffu, fabsf(reference()) > kFar && to != -INFINITY);
+                    const float f = none ? 0.0f : exp2_ftz((before - reference()) + (rest - (far ? residual() : 0.0f)));
                     l *= f;
-                    m = to;
                     if (i != first) {  // (the first product overwrites O; later ones are complete: s_full)
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
@@ -546,7 +556,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
+                float base = most == -INFINITY ? 0.0f : reference();
+                if (far) {
+                    const float from = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+                    for (int j = 0; j < kTileTokens; ++j) x[j] -= from;
+                    base = 0.0f;
+                }
                 const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), minus2 = pair_of(-base, -base);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -584,7 +600,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             float* out = p.part + ((size_t)(blockIdx.x + run) * 2 + w) * kRowsFloats;
             // (rows behind the batch are not read)
             const bool wanted = (mtile + (kDual ? 0 : w)) * kTileSeqs + row / kGroup < p.batch;
-            if (wanted) reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(m, l);
+            if (wanted) reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(reference(), l);
             if (n > first) {
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
