@@ -49,7 +49,12 @@ constexpr int kSoftmaxThreads = 256;
 constexpr int kMmaWarp = 8, kLoadWarp = 9;          // of a third warpgroup, which gives its registers
 constexpr int kPrefixThreads = 384;                 // to the other two (setmaxnreg)
 constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
-constexpr float kSlack = 8.0f;                      // weights are at most 2^8 (F16 holds 2^15)
+// Weights are at most 2^kTop, and 2^kUnit at the largest logit that moved the reference; it moves when one is 2^(kTop -
+// kUnit) above it.  F16 ends at 2^16 and keeps 11 bits down to 2^-14, so a weight keeps them down to 2^-21 of a
+// stretch's largest and is off by 2^-32 of it at most below that (with no unit, 2^-25: the tail behind one dominant
+// token was lost).  A larger unit keeps more and moves more often: 64 x 32768 takes 58.6 us with 7, 59.1 with 11,
+// 61.6 with 14 (58.4 with none).
+constexpr float kTop = 15.0f, kUnit = 7.0f;
 // Weights are 2^(logit x scale - reference), one FMA.  The reference is the largest logit's product, rounded: by 2^-4
 // at most up to 2^20, where weights may just as well be relative to it.  Behind that the rounding would leave F16's
 // range, so the difference is formed before the scale.
@@ -510,8 +515,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             // The largest logit that moved the reference, before its scale; whether any of the warp's is far; the sum.
             float most = -INFINITY, l = 0.0f;
             bool far = false;
-            const auto reference = [&]() { return __fmul_rn(most, p.scale_log2); };  // (rounded, never part of an FMA)
-            const auto residual = [&]() { return fmaf(most, p.scale_log2, -reference()); };
+            const auto reference = [&]() { return __fsub_rn(__fmul_rn(most, p.scale_log2), kUnit); };  // (rounded, never part of an FMA)
+            const auto residual = [&]() { return fmaf(most, p.scale_log2, -reference()) - kUnit; };
             const uint32_t step = kDual ? 2 : 1, first = kDual ? w : 0;
             for (uint32_t i = first; ok && i < n; i += step) {
                 ok = __all_sync(0xffffffffu, wait_phase(&s_full[w], logits_seen++ & 1, &dead));
@@ -536,7 +541,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                                                             : fmaxf(tops[i4], x[j + i4]);
                 }
                 const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-                if (__any_sync(0xffffffffu, (top - most) * p.scale_log2 > kSlack)) {
+                if (__any_sync(0xffffffffu, (top - most) * p.scale_log2 > kTop - kUnit)) {
                     const float to = fmaxf(most, top), before = reference();
                     const float rest = far ? residual() : 0.0f;
                     const bool none = most == -INFINITY;
@@ -561,7 +566,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     const float from = most == -INFINITY ? 0.0f : most;
 #pragma unroll
                     for (int j = 0; j < kTileTokens; ++j) x[j] -= from;
-                    base = 0.0f;
+                    base = -kUnit;
                 }
                 const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2), minus2 = pair_of(-base, -base);
                 uint64_t sum2[2] = {0, 0};

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import kv_oracle as ko
-from test_gpu_kv_long import pool_of
+from test_gpu_kv_long import counts_of, pool_of
 from test_gpu_kv_pages import TOL16, dev, i32
 
 pytestmark = pytest.mark.gpu
@@ -39,3 +39,47 @@ def test_shared_huge_finite_logits(cuda, batch, size):
     got = got.double().cpu().numpy()
     assert np.isfinite(got).all()
     assert np.max(np.abs(got - want)[sure]) < TOL16 * np.max(np.abs(pkv[:, 1]))
+
+
+def weighted(q, kv, counts):
+    """One query row over tokens kv [n, 2, 128] with counts: the result and sum p |v| per channel, and 1 / sum exp."""
+    x = kv[:, 0] @ q.astype(np.float64) / np.sqrt(128.0)
+    e = counts * np.exp(x - x.max())
+    p = e / e.sum()
+    return p @ kv[:, 1], p @ np.abs(kv[:, 1]), 1 / e.sum()
+
+
+def sink_and_tail(cuda, batch, heads, prefix, gaps):
+    """One token whose logit is `gap` above a flat tail of the rest and whose V is near zero: the result is the
+    tail's share.  A quarter of the rows each has its gap.  Checked on rows of the first and the last sequences."""
+    rng = np.random.default_rng(42)
+    pages = 8
+    kv = ko.rows(rng, pages * 64, heads, 0.1)
+    kv[:, 1] = (1.0 + 0.1 * rng.standard_normal(kv[:, 1].shape)).astype(np.float16)
+    kv[:, 0, :, 0] = 0.0
+    kv[0, 0, :, 0], kv[0, 1] = 1.0, 2.0**-10
+    pre, pkv = pool_of(cuda, rng, "f16", heads, pages, kv)
+    table = rng.integers(1, pages, -(-prefix // 64)).astype(np.int32)
+    table[1] = 0
+    counts = counts_of(table, prefix, pages)
+    q = (0.1 * rng.standard_normal((batch, 4 * heads, 128))).astype(np.float16)
+    q[:, :, 0] = np.tile(np.asarray(gaps) * np.sqrt(128.0), heads)
+    own, _ = pool_of(cuda, rng, "int8", heads, 1)
+    got = own.attention_shared(dev(q), i32(np.zeros((batch, 1))), i32([0] * batch), pre, i32(table), prefix)
+    own.check()
+    got = got[[0, 1, batch - 1]].double().cpu().numpy()
+    for i, b in enumerate((0, 1, batch - 1)):
+        for h in range(4 * heads):
+            want, size, inv = weighted(q[b, h], pkv[:, :, h // 4], counts)
+            yield got[i, h], want, size, inv, q[b, h], pkv[:, :, h // 4]
+
+
+@pytest.mark.parametrize("batch,prefix", [(3, 32768), (64, 32768), (1216, 4096), (1216, 32768)])
+def test_shared_tail_behind_a_dominant_token(cuda, batch, prefix):
+    """A CTA's stretch is up to 256 tiles here.  A weight is rounded by 2^-11 of itself, or by 2^-32 of the largest
+    (which is 1 / sum exp of the whole) where that is more; the result by 2^-11; a logit (|q k| summed < 21, 12
+    additions cut by 2^-23, three roundings) by 2^-18, so the mean by twice that."""
+    for got, want, size, inv, *_ in sink_and_tail(cuda, batch, 8, prefix, (8.0, 12.0, 16.0, 18.5)):
+        n = min(prefix, 32768)
+        bound = (2.0**-11 + 2 * 2.0**-18) * size + 2.0**-11 * np.abs(want) + n * 2.0**-32 * inv * 1.5 + 2.0**-25
+        assert np.all(np.abs(got - want) < bound), (np.max(np.abs(got - want) / bound), want[0])
