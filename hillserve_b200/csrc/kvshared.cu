@@ -229,9 +229,15 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
 }
 
 // A CTA's stretch of the line, one segment (its part of a run) at a time.  A run
-// takes `idle` places, then one for each tile.
+// takes `idle` places, then one for each tile.  The tensor cores cut what they add
+// to an accumulator, eight times a tile: a segment ends after kMostTiles, and its
+// sums are added with rounding to those of its run so far.  Equal weights over 2^20
+// tokens in one stretch: 4.1e-3 too little in one sum, 3e-5 so; 1216 sequences on
+// 2^20 tokens take 15.06 ms, 14.94 in one sum.
+constexpr uint32_t kMostTiles = 256;
 struct Segment {
     uint32_t u, end, idle, places;
+    bool more = false;  // of the run that the last segment had, in this stretch
     __device__ Segment(uint32_t begin, uint32_t stop, uint32_t cost, uint32_t tiles)
         : u(begin), end(stop), idle(cost), places(cost + tiles) {
         skip();
@@ -240,10 +246,12 @@ struct Segment {
     __device__ bool done() const { return u >= end; }
     __device__ uint32_t run() const { return u / places; }
     __device__ uint32_t first() const { return u % places - idle; }
-    __device__ uint32_t count() const { return min(end - u, places - u % places); }
+    __device__ uint32_t count() const { return min(min(end - u, places - u % places), kMostTiles); }
     __device__ void next() {
+        const uint32_t last = run();
         u += count();
         skip();
+        more = run() == last;
     }
 };
 
@@ -605,8 +613,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
             float* out = p.part + ((size_t)(blockIdx.x + run) * 2 + w) * kRowsFloats;
             // (rows behind the batch are not read)
             const bool wanted = (mtile + (kDual ? 0 : w)) * kTileSeqs + row / kGroup < p.batch;
-            if (wanted) reinterpret_cast<float2*>(out + kTileRows * kDim)[row] = make_float2(reference(), l);
-            if (n > first) {
+            float2* const ml = reinterpret_cast<float2*>(out + kTileRows * kDim) + row;
+            float4* const quads = reinterpret_cast<float4*>(out) + row;
+            if (!seg.more) {
+                if (wanted) *ml = make_float2(reference(), l);
+                if (n > first) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float o[32];
+                        tmem_load32(o_at + c * 32, o);
+                        tmem_wait_load();
+                        if (!wanted) continue;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            quads[(c * 8 + j) * kTileRows] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    }
+                } else if (wanted) {  // no tile for this warpgroup
+                    for (int c = 0; c < 32; ++c) quads[c * kTileRows] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            } else if (n > first) {  // added to the run's so far, which this thread wrote
+                float by = 0.0f, held = 0.0f;
+                if (wanted) {
+                    const float2 was = *ml;
+                    const float now = reference(), to = fmaxf(was.x, now);
+                    held = was.x == -INFINITY ? 0.0f : exp2_ftz(was.x - to);
+                    by = now == -INFINITY ? 0.0f : exp2_ftz(now - to);
+                    *ml = make_float2(to, fmaf(held, was.y, by * l));
+                }
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float o[32];
@@ -614,13 +647,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv_prefix_kernel(const __gr
                     tmem_wait_load();
                     if (!wanted) continue;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        reinterpret_cast<float4*>(out)[(c * 8 + j) * kTileRows + row] =
-                            make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    for (int j = 0; j < 8; ++j) {
+                        float4& sum = quads[(c * 8 + j) * kTileRows];
+                        const float4 was = sum;
+                        sum = make_float4(fmaf(held, was.x, by * o[4 * j]), fmaf(held, was.y, by * o[4 * j + 1]),
+                                          fmaf(held, was.z, by * o[4 * j + 2]), fmaf(held, was.w, by * o[4 * j + 3]));
+                    }
                 }
-            } else if (wanted) {  // no tile for this warpgroup
-                for (int c = 0; c < 32; ++c)
-                    reinterpret_cast<float4*>(out)[c * kTileRows + row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
             tc_fence_before();
             number += n;

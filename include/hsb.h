@@ -706,7 +706,7 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
  * own d_lengths[b] tokens in `pages` (any format; same kv_heads).  d_q, d_out
  * F16.  prefix_tokens >= 1; an own length may be 0.  Weights over the prefix
  * are rounded to F16: by 2^-11 of themselves, or by 2^-32 of the largest near
- * them (in their CTA's stretch) where that is more. */
+ * them (within 2^15 tokens) where that is more. */
 size_t hsb_kv_attention_shared_workspace_bytes(size_t batch, int kv_heads, size_t prefix_tokens);
 int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_table, size_t prefix_tokens,
                             const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width,

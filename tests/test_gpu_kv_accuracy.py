@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 
 import kv_oracle as ko
-from test_gpu_kv_long import counts_of, pool_of
-from test_gpu_kv_pages import TOL16, dev, i32
+from test_gpu_kv_long import attention, counts_of, pool_of
+from test_gpu_kv_pages import TOL16, close, dev, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,52 @@ def test_shared_tail_behind_a_dominant_token(cuda, batch, prefix):
         n = min(prefix, 32768)
         bound = (2.0**-11 + 2 * 2.0**-18) * size + 2.0**-11 * np.abs(want) + n * 2.0**-32 * inv * 1.5 + 2.0**-25
         assert np.all(np.abs(got - want) < bound), (np.max(np.abs(got - want) / bound), want[0])
+
+
+@pytest.mark.parametrize("heads,batch", [(8, 1216), (2, 4), (2, 64)])
+def test_shared_sum_over_a_million_tokens(cuda, heads, batch):
+    """Equal weights over 2^20 tokens with V of one sign, in stretches of 8192, 111 and 111 tiles: the tensor cores cut
+    each of a tile's eight additions to the sum (by 2^-23 of it at most, and 2^-23 within the product), so no sum goes
+    on for more than 256 tiles."""
+    rng = np.random.default_rng(43)
+    pages, prefix = 8, (1 << 20) + 77
+    kv = ko.rows(rng, pages * 64, heads)
+    kv[:, 1] = (1.0 + 0.1 * rng.standard_normal(kv[:, 1].shape)).astype(np.float16)
+    pre, pkv = pool_of(cuda, rng, "f16", heads, pages, kv)
+    table = rng.integers(0, pages, -(-prefix // 64)).astype(np.int32)
+    counts = counts_of(table, prefix, pages)
+    own, _ = pool_of(cuda, rng, "int8", heads, 1)
+    got = own.attention_shared(dev(np.zeros((batch, 4 * heads, 128), np.float16)), i32(np.zeros((batch, 1))),
+                               i32([0] * batch), pre, i32(table), prefix)
+    own.check()
+    want = np.repeat(np.tensordot(counts / counts.sum(), pkv[:, 1], 1), 4, 0)
+    bound = (2.0**-11 + 2**-18 + 256 * 8 * 2 * 2.0**-23) * np.abs(want)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert np.all(err < bound), np.max(err / np.abs(want))
+
+
+@pytest.mark.parametrize("heads,batch,prefix", [(8, 1216, 33000), (8, 1216, 70000), (1, 9472, 40000)])
+def test_shared_stretches_in_several_sums(cuda, heads, batch, prefix):
+    """Stretches that begin and end their sums several times: logits that rise from page to page, the dominant part in
+    the first, the last or all of them, a bad page among them."""
+    rng = np.random.default_rng(44)
+    pages = 32
+    kv = ko.rows(rng, pages * 64, heads)
+    kv[:, 0, :, 0] = (np.arange(pages * 64) // 64 * 1.0)[:, None]
+    pre, pkv = pool_of(cuda, rng, "f16", heads, pages, kv)
+    total = -(-prefix // 64)
+    table = (np.arange(total) * pages // total).astype(np.int32)
+    table[total // 2] = -1
+    counts = counts_of(table, prefix, pages)
+    q = rng.standard_normal((batch, 4 * heads, 128)).astype(np.float16)
+    q[:, :, 0] = np.tile(np.array([1.0, -1.0, 0.0, 0.5]) * np.sqrt(128.0), heads)
+    own, okv = pool_of(cuda, rng, "int8", heads, 1)
+    got = own.attention_shared(dev(q), i32(np.zeros((batch, 1))), i32([3] * batch), pre, i32(table), prefix)
+    with pytest.raises(cuda.InvalidArgument) as e:
+        own.check()
+    assert e.value.status == 121
+    both, pick = np.concatenate([pkv, okv]), sorted(rng.choice(batch, 20, replace=False)) + [batch - 1]
+    counts = np.concatenate([counts, np.arange(64) < 3])
+    want = np.stack([attention(q[b], both, counts) for b in pick])
+    # (|logit| < 32 + 16: fifteen roundings of 2^-23 each, twice)
+    close(got[pick], want, [both], TOL16 + 256 * 8 * 2 * 2.0**-23 + 2 * 15 * 2.0**-23 * 48)
