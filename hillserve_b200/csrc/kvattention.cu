@@ -18,8 +18,9 @@
 // at no cost.  Which channel sits at which k (or row) of the MMA is free, as
 // long as both operands agree: each lane owns whole 16-byte chunks, so the
 // fragments are the loaded words themselves, with no ldmatrix.  The K scale
-// multiplies a token's logits, the V scale its weight, both in F32; weights
-// are brought into F16's range by a power of two before their split into halves.
+// multiplies a token's logits, the V scale its weight, both in F32; the largest
+// weights are brought into F16's range by a power of two before their split into
+// halves, so a weight is off by 2^-22 of itself, or 2^-32 of a head's largest.
 // The running maximum is only moved when a logit passes it by 8 (in log2): until
 // then no reduction across the warp and no rescaling is needed.
 //
@@ -47,10 +48,14 @@
 namespace hsb {
 namespace {
 
-// Weights enter the second product as p x 2^7 (x the V scale over its
-// reference): p is at most 2^kSlack, so their F16 halves reach 2^15 at most.
-constexpr float kWeightUnit = 128.0f;
+// Weights enter the second product times a unit.  F16: 2^7, and p is at most
+// 2^kSlack, so their halves reach 2^15 at most.  8 bits: p x V scale, the unit
+// a power of two that brings the largest such weight so far to 2^7 and moves when
+// one would pass 2^15.  (Taken from the scales alone, it would follow rows that
+// the softmax ignores: one of 6e4 among 1e-3 cost the others 14 of their 22 bits.)
+constexpr float kWeightUnit = 128.0f, kTopWeight = 32768.0f;
 constexpr float kSlack = 8.0f;
+constexpr float kFirstUnit = 0x1p100f, kLeastWeight = 0x1p-93f;  // before any weight; kWeightUnit / kFirstUnit
 
 // Each warp's ring holds K and V of its units in turn (K 0, V 0, K 1, ...): a
 // slot is free again as soon as its product is done.  A unit is a page in 8
@@ -104,6 +109,16 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
+// The maximum over the lanes of this one's columns (t, t ^ 2), which hold all rows of a unit: two reductions by
+// the warp, 0.2 us less in a run's first unit than four exchanges.
+__device__ __forceinline__ float rows_max(float v, bool odd) {
+    float a, b;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(a) : "f"(odd ? -INFINITY : v));
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(b) : "f"(odd ? v : -INFINITY));
+    return odd ? b : a;
+}
+// 1 / x of a normal power of two below 2^127 (a run of 77 tokens 5.0 us, with divisions 5.5).
+__device__ __forceinline__ float inverse_of_power(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 __device__ __forceinline__ float lds32(uint32_t addr) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
@@ -350,7 +365,9 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         // ================ one run, as far as it lies in this part
         const uint32_t begin = k.u, run_begin = k.run, run_end = k.run_end(), tokens = k.tokens;
         const uint32_t stop = min(run_end, k.end), run = k.seq * p.v.heads + k.head;
-        float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f}, vref = 0.0f, vunit = Fmt::kScaled ? 0.0f : kWeightUnit;
+        float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
+        constexpr float kUnit0 = Fmt::kScaled ? kFirstUnit : kWeightUnit;
+        float unit[2] = {kUnit0, kUnit0};
         float o[8][4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
@@ -455,39 +472,47 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
                 }
                 bool grown = false;
 #pragma unroll
-                for (int e = 0; e < kTiles; ++e) {
-                    grown |= x[0][e] > M[0] + kSlack || x[1][e] > M[1] + kSlack;
-                    if constexpr (Fmt::kScaled) grown |= vs[e] > vref;
-                }
-                if (__any_sync(0xffffffffu, grown)) {
-                    // move the maxima (of both lanes' rows) and the power of two over the V scales
-                    float fold[2], vfold = 1.0f;
-                    if constexpr (Fmt::kScaled) {
-                        float top = 0.0f;
-#pragma unroll
-                        for (int e = 0; e < kTiles; ++e) top = fmaxf(top, vs[e]);
-                        top = warp_max(top);
-                        const float up = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0xff800000u);
-                        if (up > vref) {
-                            vfold = vref / up;
-                            vref = up;
-                            vunit = kWeightUnit / up;
-                        }
-                    }
+                for (int e = 0; e < kTiles; ++e) grown |= x[0][e] > M[0] + kSlack || x[1][e] > M[1] + kSlack;
+                grown = __any_sync(0xffffffffu, grown);
+                float fold[2] = {1.0f, 1.0f};
+                if (grown) {  // move the maxima (of both lanes' rows)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float top = x[j][0];
 #pragma unroll
                         for (int e = 1; e < kTiles; ++e) top = fmaxf(top, x[j][e]);
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        top = fmaxf(top, M[j]);
+                        top = fmaxf(rows_max(top, t & 1), M[j]);
                         fold[j] = M[j] == -INFINITY ? 0.0f : exp2_ftz(M[j] - top);
                         L[j] *= fold[j];
-                        fold[j] *= vfold;
                         M[j] = top;
+                    }
+                }
+                const float base0 = M[0] == -INFINITY ? 0.0f : M[0], base1 = M[1] == -INFINITY ? 0.0f : M[1];
+                bool over = false;
+#pragma unroll
+                for (int e = 0; e < kTiles; ++e) {
+                    const float p0 = exp2_ftz(x[0][e] - base0), p1 = exp2_ftz(x[1][e] - base1);
+                    L[0] += p0;
+                    L[1] += p1;
+                    x[0][e] = Fmt::kScaled ? p0 * vs[e] : p0;
+                    x[1][e] = Fmt::kScaled ? p1 * vs[e] : p1;
+                    if constexpr (Fmt::kScaled) over |= x[0][e] * unit[0] > kTopWeight || x[1][e] * unit[1] > kTopWeight;
+                }
+                if constexpr (Fmt::kScaled) over = __any_sync(0xffffffffu, over);
+                if (grown || over) {
+                    // the sums' new references: the maxima, and in 8 bits units for the largest weight so far
+                    if constexpr (Fmt::kScaled) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float top = x[j][0];
+#pragma unroll
+                            for (int e = 1; e < kTiles; ++e) top = fmaxf(top, x[j][e]);
+                            const float held = fold[j] * (kWeightUnit * inverse_of_power(unit[j]));
+                            top = fmaxf(fmaxf(rows_max(top, t & 1), held), kLeastWeight);
+                            const float up = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0xff800000u);
+                            fold[j] = held * inverse_of_power(up);
+                            unit[j] = kWeightUnit * inverse_of_power(up);
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -497,17 +522,13 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
                         o[j][3] *= fold[1];
                     }
                 }
-                const float base0 = M[0] == -INFINITY ? 0.0f : M[0], base1 = M[1] == -INFINITY ? 0.0f : M[1];
                 uint32_t bp[2 * kTiles];  // P^T fragments of rows i
 #pragma unroll
                 for (int e = 0; e < kTiles; ++e) {
-                    const float p0 = exp2_ftz(x[0][e] - base0), p1 = exp2_ftz(x[1][e] - base1);
-                    L[0] += p0;
-                    L[1] += p1;
-                    const float unit = Fmt::kScaled ? vs[e] * vunit : kWeightUnit;
-                    const __half2 hi = __floats2half2_rn(p0 * unit, p1 * unit);
+                    const float w0 = x[0][e] * unit[0], w1 = x[1][e] * unit[1];
+                    const __half2 hi = __floats2half2_rn(w0, w1);
                     const float2 f = __half22float2(hi);
-                    const __half2 lo = __floats2half2_rn(p0 * unit - f.x, p1 * unit - f.y);
+                    const __half2 lo = __floats2half2_rn(w0 - f.x, w1 - f.y);
                     const uint32_t hw = *reinterpret_cast<const uint32_t*>(&hi), lw = *reinterpret_cast<const uint32_t*>(&lo);
                     const uint32_t keep = low ? lw : hw, other = __shfl_xor_sync(0xffffffffu, low ? hw : lw, 2);
                     bp[e] = transpose_8x8(low ? other : keep);
@@ -572,8 +593,8 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
         if (!k.done()) load_query();
         // ---------------- the run's end here: all rows' sums, rounding + remainder.  Lanes t < 2
         // keep head h0, lanes t >= 2 head h0 + 1, and give the other's parts away.
-        const float os = Fmt::kScaled ? vref / kWeightUnit : 1.0f / kWeightUnit;
         const int h = h0 + low;
+        const float os = inverse_of_power(low ? unit[1] : unit[0]);
         const float top = low ? M[1] : M[0];
         float sum = (low ? L[1] : L[0]) + __shfl_xor_sync(0xffffffffu, low ? L[0] : L[1], 2);
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);

@@ -695,7 +695,9 @@ int hsb_kv_read(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_
  * [batch][4 kv_heads][128], out = softmax(q . K / sqrt(128)) V over positions
  * [0, d_lengths[b]); zero for an empty sequence.  Grids depend on batch and
  * table_width only, so a captured call follows lengths and tables as they
- * change.  Workspace: as for the other stages, of one call at a time. */
+ * change.  Workspace: as for the other stages, of one call at a time.  A weight
+ * (in 8 bits times its V scale) is off by 2^-21 of itself, or by 2^-31 of the
+ * head's largest where that is more. */
 size_t hsb_kv_attention_workspace_bytes(size_t batch, int kv_heads);
 int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t table_width, const int32_t* d_lengths,
                      size_t batch, const float* d_q, float* d_out, void* d_workspace, size_t workspace_bytes,

@@ -7,7 +7,7 @@ import pytest
 
 import kv_oracle as ko
 from test_gpu_kv_long import attention, counts_of, pool_of
-from test_gpu_kv_pages import TOL16, close, dev, i32
+from test_gpu_kv_pages import TOL16, close, dev, i32, quick_fill
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,60 @@ def test_shared_stretches_in_several_sums(cuda, heads, batch, prefix):
     want = np.stack([attention(q[b], both, counts) for b in pick])
     # (|logit| < 32 + 16: fifteen roundings of 2^-23 each, twice)
     close(got[pick], want, [both], TOL16 + 256 * 8 * 2 * 2.0**-23 + 2 * 15 * 2.0**-23 * 48)
+
+
+# ------------------------------------------------------------ paged attention
+def strict(got, q, kv, top):
+    """One sequence's rows against 64 bits, channel by channel.  With s a row's V scale (1 in F16), a weight is off by
+    2^-21 of itself (two halves of 11 bits, three roundings) or by 2^-31 of the head's largest weight x scale where
+    that is more, but no weight by more than itself; with S = sum |q k| / sqrt(128) < 16 and |logit| < 32 of every
+    row that counts, exp by 2e-5 (test_gpu_kv_pages.py) and so the mean by twice that."""
+    got, worst = got.double().cpu().numpy(), 0.0
+    for h in range(len(q)):
+        k, v = kv[:, 0, h // 4], kv[:, 1, h // 4]
+        x = k @ q[h].astype(np.float64) / np.sqrt(128.0)
+        p = np.exp(x - x.max())
+        s = np.max(np.abs(v), axis=1) / top if top else np.ones(len(v))
+        off = 2.0**-21 * p + np.minimum(p, 2.0**-31 * np.max(p * s) / np.maximum(s, 1e-30))
+        bound = (4e-5 * p + off) @ np.abs(v) / p.sum()
+        worst = max(worst, np.max(np.abs(got[h] - p @ v / p.sum()) / np.maximum(bound, 1e-30)))
+    assert worst < 1.0, worst
+
+
+TOPS = {"f16": None, "int8": 127.0, "e4m3": 448.0}
+
+
+@pytest.mark.parametrize("fmt", ko.FORMATS)
+@pytest.mark.parametrize("n,at", [(513, 0), (513, 70), (513, 512), (4000, 1), (4000, 3000)])
+@pytest.mark.parametrize("gap", [-20.0, -30.0, -60.0])
+def test_loud_rows_that_count_little(cuda, fmt, n, at, gap):
+    """One V of 6e4 among others of 1e-3, its logit far below theirs (or theirs far above it, where it comes first)."""
+    rng = np.random.default_rng(45)
+    kv = ko.rows(rng, n, 2)
+    kv[:, 0, :, 0] = 0.0
+    kv[:, 1] = (kv[:, 1].astype(np.float32) * 1e-3).astype(np.float16)
+    kv[at, 0, :, 0] = gap
+    kv[at, 1] = np.clip(rng.standard_normal((2, 128)) * 3e4, -6e4, 6e4).astype(np.float16)
+    table, pages = ko.tables(rng, [n])
+    cache = cuda.KVPages(pages=pages, kv_heads=2, format=fmt)
+    cache.append(dev(kv), i32(table), i32([0]), offsets=i32([0, n]))
+    q = (0.5 * rng.standard_normal((1, 8, 128))).astype(np.float32)
+    q[:, :, 0] = np.sqrt(128.0)
+    got = cache.attention(dev(q), i32(table), i32([n]))
+    cache.check()
+    strict(got[0], q[0], ko.stored(kv, fmt), TOPS[fmt])
+
+
+@pytest.mark.parametrize("fmt", ko.FORMATS)
+@pytest.mark.parametrize("lengths", [[77], [20011], [500, 1, 2048, 0, 777, 4096], [33] * 40])
+def test_attention_channel_by_channel(cuda, fmt, lengths):
+    rng = np.random.default_rng(46)
+    cache, table, kvs = quick_fill(cuda, rng, fmt, 4, lengths)
+    q = (0.7 * rng.standard_normal((len(lengths), 16, 128))).astype(np.float32)
+    got = cache.attention(dev(q), i32(table), i32(lengths))
+    cache.check()
+    for b, kv in enumerate(kvs):
+        if len(kv):
+            strict(got[b], q[b], kv, TOPS[fmt])
+        else:
+            assert not got[b].any()
