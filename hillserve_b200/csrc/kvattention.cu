@@ -698,9 +698,10 @@ __global__ void __launch_bounds__(Ring<F>::kThreads, 1) kv_attention_kernel(cons
 // does not end there, in the order of the CTAs (a run that goes on leaves no
 // empty stretch before its end): head blockIdx.y, thread = channel.  Every load
 // of the first 32 partials' weights and 8 outputs is on its way before the
-// run's extent is known; what lies behind it is not used.
-__global__ void __launch_bounds__(kDim) kv_combine_kernel(const float* __restrict__ part, const RunInfo* __restrict__ infos,
-                                                         float* __restrict__ out) {
+// run's extent is known; what lies behind it is not used.  The kernel may be
+// resident while its partials are written: no pointer promises constant data,
+// so that no load may pass the wait.
+__global__ void __launch_bounds__(kDim) kv_combine_kernel(const float* part, const RunInfo* infos, float* out) {
     constexpr int kFirst = 8;
     pdl_trigger();
     pdl_wait();
