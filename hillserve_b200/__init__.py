@@ -747,18 +747,23 @@ class KVPages:
         self._i32, self._f16, self._f32 = torch.int32, torch.float16, torch.float32
         self._like = torch.empty_like
         self._device_of, self._stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-        self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            self.status = torch.zeros(2, dtype=torch.int32, device=self.device)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()  # zero before a call on any stream
         self._c = KvPages(data.data_ptr(), self.pages, self.FORMATS[format], self.kv_heads)
         self._ref, self._st = C.byref(self._c), self.status.data_ptr()
 
     def check(self, stream=None) -> None:
-        """Synchronises; raises (and forgets) what the calls so far recorded."""
-        try:
-            with _torch().cuda.device(self.device):
-                _check_status(self.status, stream if stream is not None else _torch().cuda.current_stream(self.device))
-        except HsbError:
-            self.status.zero_()
-            raise
+        """Waits for the device, or only for ``stream``; raises, and forgets, the
+        first of what calls on it recorded.  A call still in flight on another
+        stream loses nothing by that."""
+        torch = _torch()
+        with torch.cuda.device(self.device):
+            if stream is None:
+                torch.cuda.synchronize()
+                stream = torch.cuda.current_stream()
+            _raise(self._lib.hsb_status_take(self._st, stream.cuda_stream))
 
     def _arg(self, t, name: str, dtype, shape: tuple) -> int:
         """Address of a contiguous tensor of this type and shape on the pool's device."""

@@ -57,6 +57,7 @@ _SIGNATURES = {
     "hsb_last_error": (C.c_char_p, []),
     "hsb_status_message": (C.c_char_p, [I]),
     "hsb_status_check": (I, [P, P]),
+    "hsb_status_take": (I, [P, P]),
     "hsb_score_v3": (I, [P, P, SZ, SZ, P, P]),
     "hsb_score_views": (I, [P, P, SZ, P, P]),
     "hsb_score_pipeline_v3": (I, [P, P, C.c_uint32, P, P]),

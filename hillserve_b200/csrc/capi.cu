@@ -39,6 +39,10 @@ DeviceInfo g_devices[64];
 std::atomic<bool> g_device_ready[64];
 }  // namespace
 
+namespace {
+__global__ void status_clear_kernel(unsigned long long* word, unsigned long long seen) { atomicCAS(word, seen, 0ull); }
+}  // namespace
+
 int record_error(int status, const char* message) { return fail(status, message); }
 int record_cuda_error(cudaError_t e, const char* what) { return fail_cuda(e, what); }
 
@@ -143,6 +147,24 @@ int hsb_status_check(const hsb_device_status* d_status, void* stream) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(as_stream(stream));
     if (e != cudaSuccess) return fail_cuda(e, "status read-back");
     if (h.code) return fail(h.code, hsb_status_message(h.code));
+    g_last_error.clear();
+    return HSB_OK;
+}
+
+int hsb_status_take(hsb_device_status* d_status, void* stream) {
+    if (!d_status || !aligned(d_status, 8)) return fail(HSB_E_INVALID, "null or misaligned status");
+    unsigned long long seen = 0;  // code in the low half, index in the high one
+    static_assert(sizeof(seen) == sizeof(hsb_device_status), "one word");
+    cudaError_t e = cudaMemcpyAsync(&seen, d_status, sizeof(seen), cudaMemcpyDeviceToHost, as_stream(stream));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(as_stream(stream));
+    const int code = (int)(seen & 0xffffffffull);
+    if (e == cudaSuccess && code) {
+        status_clear_kernel<<<1, 1, 0, as_stream(stream)>>>(reinterpret_cast<unsigned long long*>(d_status), seen);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = cudaStreamSynchronize(as_stream(stream));
+    }
+    if (e != cudaSuccess) return fail_cuda(e, "status read-back");
+    if (code) return fail(code, hsb_status_message(code));
     g_last_error.clear();
     return HSB_OK;
 }

@@ -131,6 +131,10 @@ typedef struct hsb_device_status {
 /* Synchronises `stream`, reads *d_status, sets the last-error message and
  * returns the status it holds.  Does not clear it. */
 int hsb_status_check(const hsb_device_status* d_status, void* stream);
+/* The same, and clears what it returns before it returns it.  What a call in
+ * flight on another stream records meanwhile stays for the next look (where it
+ * comes before what was returned: the word holds the first). */
+int hsb_status_take(hsb_device_status* d_status, void* stream);
 
 /* ------------------------------------------------------------------ stage 1
  * Replaces FullGqaCpuScorer::score (policy/full_gqa_cpu.hpp:43-45,

@@ -50,3 +50,13 @@ def test_a_cut_run_keeps_its_partials(ask):
     assert all(w for w, (f, c) in zip(words, cuts) if (f, c) != (0, 0))
     for (_, count), (n,) in zip(cuts, ask([f"place {w} 148" for w in words])):
         assert n == count
+
+
+def test_status_take_refuses():
+    import ctypes as C
+
+    from hillserve_b200 import _capi
+
+    lib = _capi.lib()
+    for at in (None, C.c_void_p(0x10004)):
+        assert lib.hsb_status_take(at, None) == lib.hsb_status_check(None, None) != 0
