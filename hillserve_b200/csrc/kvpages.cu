@@ -117,8 +117,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
             seq = sequence_of(p.offsets, p.batch, row);
             if (seq >= 0) first = p.offsets[seq];
         }
-        if (seq >= 0) {
-            const unsigned long long pos = (unsigned long long)(uint32_t)p.starts[seq] + (unsigned long long)(row - first);
+        const int32_t start = seq >= 0 ? p.starts[seq] : 0;
+        if (start < 0) {  // (no position at all, however wide the table)
+            raise_status(p.status, HSB_E_KV_POSITION, (int)row);
+        } else if (seq >= 0) {
+            const unsigned long long pos = (unsigned long long)start + (unsigned long long)(row - first);
             const long long page = page_of(p.v, seq, pos, p.status, (int)row);
             if (page >= 0) at = page * kPageTokens + (long long)(pos % kPageTokens);
         }

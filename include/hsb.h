@@ -647,8 +647,8 @@ int hsb_executor_decode_layer(const uint16_t* d_current, const float* d_rehearsa
  *
  * Position t of sequence b lives in row t % 64 of page d_table[b * table_width
  * + t / 64].  Entries behind a sequence's last page are not read.  An entry
- * outside the pool sets HSB_E_KV_PAGE, a position or length behind the table's
- * end HSB_E_KV_POSITION, in *d_status (index = the row or sequence; d_status
+ * outside the pool sets HSB_E_KV_PAGE, a negative start or length, or a position
+ * or length behind the table's end, HSB_E_KV_POSITION, in *d_status (index = the row or sequence; d_status
  * may be NULL): nothing outside the pool or the table is touched, the row is
  * skipped (written) or zero (read), the page's tokens are left out of the
  * attention, and a sequence of such a length counts as empty.
