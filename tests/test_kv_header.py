@@ -60,3 +60,17 @@ def test_status_take_refuses():
     lib = _capi.lib()
     for at in (None, C.c_void_p(0x10004)):
         assert lib.hsb_status_take(at, None) == lib.hsb_status_check(None, None) != 0
+
+
+@pytest.mark.parametrize("n", [1, 2, 16, 148, 1184])
+def test_the_split_as_compiled(ask, n):
+    """Stretches follow one another over all units, differ by one unit at most, the longer ones first; the stretch of
+    a unit is the one that holds it.  Up to the units of 2^27 table entries of 8 heads in halves, and their run costs."""
+    rng = random.Random(n)
+    units = [1, 2, 7, 147, 148, 149, 1000, 4096 * 8 + 3, (1 << 31) + (1 << 24)] + [rng.randrange(1, 1 << 31) for _ in range(20)]
+    asked = [sorted({0, u - 1, u // 2, u // 3, min(u - 1, 5)} | {rng.randrange(u) for _ in range(20)}) for u in units]
+    for u, at, got in zip(units, asked, ask([f"split {u} {n} " + " ".join(map(str, a)) for u, a in zip(units, asked)])):
+        begins, of = got[:n + 1], got[n + 1:]
+        sizes = [b - a for a, b in zip(begins, begins[1:])]
+        assert begins[0] == 0 and begins[-1] == u and sizes == sorted(sizes, reverse=True) and sizes[0] - sizes[-1] <= 1
+        assert len(of) == len(at) and all(begins[c] <= x < begins[c + 1] for c, x in zip(of, at))
