@@ -808,9 +808,14 @@ int hsb_kv_attention(const hsb_kv_pages* pages, const int32_t* d_table, size_t t
     if (!aligned_to(16, d_q, d_out, static_cast<unsigned char*>(d_workspace)) || !aligned_to(4, d_table, d_lengths) ||
         !aligned_to(8, d_status))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
-    if (d_out == d_q) return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
-    if (!d_workspace || workspace_bytes < hsb_kv_attention_workspace_bytes(batch, pages->kv_heads))
+    const size_t bytes = batch * pages->kv_heads * kGroup * kDim * sizeof(float);
+    if (!apart(d_q, bytes, d_out, bytes))
+        return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
+    const size_t needed = hsb_kv_attention_workspace_bytes(batch, pages->kv_heads);
+    if (!d_workspace || workspace_bytes < needed)
         return record_error(HSB_E_WORKSPACE, "paged KV attention workspace missing or too small");
+    if (!apart(d_workspace, needed, d_q, bytes) || !apart(d_workspace, needed, d_out, bytes))
+        return record_error(HSB_E_KV_SHAPE, "paged KV attention workspace must not alias the query or the output");
     PagedAttention p{};
     p.v = paged_view(*pages, d_table, table_width, table_width);
     p.lengths = d_lengths;

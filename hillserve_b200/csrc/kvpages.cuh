@@ -87,6 +87,11 @@ template <typename... P>
 bool aligned_to(uintptr_t by, const P*... at) {
     return ((... | reinterpret_cast<uintptr_t>(at)) & (by - 1)) == 0;
 }
+// Whether two ranges have no byte in common.
+inline bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x >= a_bytes : x - y >= b_bytes;
+}
 PagedView paged_view(const hsb_kv_pages& p, const int32_t* table, size_t width, size_t pitch);
 
 }  // namespace hsb

@@ -870,12 +870,16 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     if (!aligned_to(16, d_q, d_out, static_cast<unsigned char*>(d_workspace)) ||
         !aligned_to(4, d_prefix_table, d_table, d_lengths) || !aligned_to(8, d_status))
         return record_error(HSB_E_KV_SHAPE, "paged KV attention buffers are misaligned");
-    if (d_out == d_q) return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
+    const size_t bytes = batch * pages->kv_heads * kGroup * kDim * sizeof(uint16_t);
+    if (!apart(d_q, bytes, d_out, bytes))
+        return record_error(HSB_E_KV_SHAPE, "paged KV attention output must not alias the query");
     const Geometry g = geometry(batch, pages->kv_heads, prefix_tokens);
     if ((unsigned long long)g.runs * (g.tiles + 4) > 0x7fffffffull)
         return record_error(HSB_E_KV_SHAPE, "paged KV attention shape");
     if (!d_workspace || workspace_bytes < g.total)
         return record_error(HSB_E_WORKSPACE, "paged KV attention workspace missing or too small");
+    if (!apart(d_workspace, g.total, d_q, bytes) || !apart(d_workspace, g.total, d_out, bytes))
+        return record_error(HSB_E_KV_SHAPE, "paged KV attention workspace must not alias the query or the output");
     unsigned char* ws = static_cast<unsigned char*>(d_workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 

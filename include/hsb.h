@@ -654,8 +654,8 @@ int hsb_executor_decode_layer(const uint16_t* d_current, const float* d_rehearsa
  * attention, and a sequence of such a length counts as empty.
  *
  * Queries, outputs, rows and workspaces are 16-byte aligned, tables, lengths
- * and positions 4-byte, d_status 8-byte; an attention's output is not its
- * query.  Limits of the attention calls: batch 2^20, batch * table_width 2^27,
+ * and positions 4-byte, d_status 8-byte; an attention's query, output and
+ * workspace do not overlap.  Limits of the attention calls: batch 2^20, batch * table_width 2^27,
  * prefix_tokens 2^30 (HSB_E_KV_SHAPE behind them).  A NaN in a query makes that
  * head's row NaN; a NaN in an attended K or V row (an F16 pool keeps them) the
  * rows of that sequence and KV head that it enters, and so may an infinity. */

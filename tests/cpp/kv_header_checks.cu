@@ -3,6 +3,7 @@
 //   split UNITS N U...   the stretches' begins (N + 1 of them), then the stretch of each U
 //   place WORD GRID      the partials that a run's place word stands for
 //   cut FIRST COUNT      the place word of a cut run
+//   apart A N B M        whether N bytes at A and M bytes at B have none in common
 #include <cstdio>
 #include <iostream>
 #include <sstream>
@@ -24,6 +25,11 @@ int main() {
             std::printf("\n");
         } else if (what == "place") {
             std::printf("%u\n", hsb::run_partials(a, b));
+        } else if (what == "apart") {
+            unsigned c = 0, d = 0;
+            in >> c >> d;
+            const auto at = [](unsigned x) { return reinterpret_cast<const void*>((uintptr_t)x); };
+            std::printf("%d\n", hsb::apart(at(a), b, at(c), d) ? 1 : 0);
         } else if (what == "cut") {
             std::printf("%u\n", hsb::cut_run(a, b));
         }

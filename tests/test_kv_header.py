@@ -74,3 +74,37 @@ def test_the_split_as_compiled(ask, n):
         sizes = [b - a for a, b in zip(begins, begins[1:])]
         assert begins[0] == 0 and begins[-1] == u and sizes == sorted(sizes, reverse=True) and sizes[0] - sizes[-1] <= 1
         assert len(of) == len(at) and all(begins[c] <= x < begins[c + 1] for c, x in zip(of, at))
+
+
+def test_ranges_apart(ask):
+    cases = [(a, n, b, m) for a in (100, 160) for n in (1, 16, 60, 61) for b in (80, 99, 100, 116, 160, 161, 220, 221)
+             for m in (1, 20, 21, 80, 81)]
+    for (a, n, b, m), (got,) in zip(cases, ask([f"apart {a} {n} {b} {m}" for a, n, b, m in cases])):
+        assert got == (not set(range(a, a + n)) & set(range(b, b + m))), (a, n, b, m)
+
+
+def test_overlapping_buffers_are_refused():
+    """An attention's output inside its query, its workspace over either: all refused before any launch."""
+    import ctypes as C
+
+    from hillserve_b200 import _capi
+
+    lib, batch, heads, base = _capi.lib(), 3, 2, 1 << 30
+    P = C.c_void_p(1 << 20)
+    at = lambda x: C.c_void_p(base + x)  # noqa: E731
+    own = C.byref(_capi.KvPages(1 << 21, 4, 1, heads))
+    pre = C.byref(_capi.KvPages(1 << 22, 4, 0, heads))
+    for width, size, call in (
+            (4, lib.hsb_kv_attention_workspace_bytes(batch, heads),
+             lambda q, o, w, n: lib.hsb_kv_attention(own, P, 4, P, batch, q, o, w, n, None, None)),
+            (2, lib.hsb_kv_attention_shared_workspace_bytes(batch, heads, 100),
+             lambda q, o, w, n: lib.hsb_kv_attention_shared(pre, P, 100, own, P, 4, P, batch, q, o, w, n, None, None))):
+        bytes_ = batch * 4 * heads * 128 * width
+        far = at(1 << 28)
+        for off in (0, 16, bytes_ - 16, 16 - bytes_):
+            assert call(at(0), at(off), far, size) == 120
+            assert lib.hsb_last_error() == b"paged KV attention output must not alias the query"
+        for ws in (at(0), at(bytes_ - 16), at(-16 * (size // 16 - 1))):
+            for q, o in ((at(0), far), (far, at(0))):
+                assert call(q, o, ws, size) == 120
+                assert lib.hsb_last_error() == b"paged KV attention workspace must not alias the query or the output"
