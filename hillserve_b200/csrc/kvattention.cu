@@ -34,12 +34,13 @@
 // F32 partials that kv_combine_kernel folds in order.
 //
 // Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences of up
-// to 8192 int8 tokens 98.0 us, 5.6 TB/s; 64 x 32768 F16, two heads, 89.1 us,
-// 6.0 TB/s (a copy reaches 6.5); one sequence of 32768 int8 tokens 20.7 us, of
-// which 10.6 are its bytes, 3.4 kv_combine_kernel (4 to 5 of the longer calls) and
-// the rest the launch and the look-ups before the first byte.  Under the profiler (e4m3, 16 x 16384) the kernel
-// reads 554 MB, the pages' bytes once, at 5.9 TB/s; 889 instructions a warp and
-// page leave the issue slots two thirds idle.
+// to 8192 int8 or e4m3 tokens 99 us, 5.6 TB/s, of up to 32768 360 us, 6.1; 64 x
+// 32768 F16, one head, 89.3 us, 6.0 TB/s (a copy reaches 6.5); one sequence of
+// 32768 int8 tokens 20.5 us, of which 10.6 are its bytes, 3.4 kv_combine_kernel
+// (4 to 5 of the longer calls) and the rest the launch and the look-ups before
+// the first byte.  Under the profiler (e4m3, 16 x 16384) the kernel reads 554 MB,
+// the pages' bytes once, at 5.8 TB/s; 910 instructions a warp and page leave the
+// issue slots two thirds idle.
 #include <algorithm>
 #include <cmath>
 
@@ -769,9 +770,10 @@ cudaError_t launch_format(int format, const PagedAttention& p, unsigned grid, cu
 
 // A CTA a run needs no scan of the lengths, no partials and no second launch, but
 // its eight warps are all that a run gets.  int8, 8 heads, by runs and split: one
-// sequence of 77 tokens (e4m3) 5.3 and 8.0 us, 512 8.0 and 9.2, 1000 10.6 and 10.0,
-// 2000 15.6 and 10.8; sixteen of up to 1000 11.1 and 15.5, 2000 17.5 and 19.0, 4000
-// 26.8 and 23.2.
+// sequence of 77 tokens (e4m3) 4.9 and 7.4 us, 512 7.7 and 8.1, 1000 10.3 and 9.5,
+// 2000 15.3 and 10.2; sixteen of up to 1000 10.8 and 14.7, 2000 17.2 and 17.8, 4000
+// 27.0 and 22.5.  The host knows the tables' width, not the lengths: short
+// sequences in wide tables are split too.
 bool paged_by_run(size_t batch, size_t table_width, int heads) {
     const size_t runs = batch * heads, sms = device_info().sms;
     return runs <= sms && table_width <= (2 * runs >= sms ? 32 : 12);

@@ -15,20 +15,22 @@
 // Two warpgroups own one M tile each: thread = row reads its 128 logits from
 // tensor memory, forms the weights without any exchange and writes them back
 // as F16 over the logits; while one softmax runs, the other tile's products do.
+// The next logits go over those weights once the product that reads them is done.
 // For at most 32 sequences there is one M tile, and the two warpgroups take the
 // even and the odd tokens' tiles of it instead.
 //
 // The (KV head, M tiles, token tile) units are split evenly over the SMs; each
-// stretch of a run leaves F32 partials.  A stretch that ends one run and begins
+// stretch of a run leaves F32 partials, summed in parts of 256 tiles.  A stretch that ends one run and begins
 // the next pays for a second query tile and a second result, so long lines keep
 // idle places for that before each run.  The sequences' own tokens go through
 // the paged kernel (kvattention.cu), and kv_shared_combine_kernel folds both.
 //
 // Measured (B200, 8 KV heads, one call in a captured graph): 64 sequences on 32768
-// tokens 55.4 us, 256 on 16461 88 to 94, 8 on 4097 14.2.  A unit (two M tiles, 128
-// tokens) takes a SM 1.76 us where the prefix stays in L2 (256 sequences), with no
-// waits for the weights 1.38, 1.8 PFLOP/s over the chip; where it comes from memory
-// (64 sequences) 1.95, its bytes alone 1.40.  192 KB of shared memory are read a
+// tokens 58.2 us, 256 on 16461 94 to 100, 8 on 4097 14.5.  A unit (two M tiles, 128
+// tokens) takes a SM 1.86 us where the prefix stays in L2 (256 sequences; 1.76 if
+// the logits did not wait for the product before), with no waits for the weights
+// either 1.38, 1.8 PFLOP/s over the chip; where it comes from memory (64 sequences)
+// 1.95, its bytes alone 1.40.  192 KB of shared memory are read a
 // unit and 64 KB written, as many cycles (2048) as the products take at best.
 // Half-width logits, twice as many softmax warps, weights handed over in smaller
 // parts, and a pair of SMs on one tile gained nothing.  Around that loop the prefix
@@ -193,9 +195,9 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // 2^y = 2^n 2^f with n the nearest integer (adding 1.5 2^23 rounds to it) and
 // 2^f on [-0.5, 0.5] a polynomial of degree 4, fitted for the least largest
 // relative error (2.7e-6; a weight is rounded to F16 by 5e-4 next).  256 x 16461
-// takes 91.3 us with every fourth pair, 93.8 with every eighth, 93.2 with none; a
+// takes 94.4 us with every fourth pair, 97.2 with every eighth, 95.8 with none; a
 // single M tile, where nothing runs beside a tile's softmax but the other tokens',
-// 15.6 (8 x 4097) and 15.2 with none.
+// 14.7 (8 x 4097) and 14.5 with none.
 constexpr int kByPolynomial = 4;
 __device__ __forceinline__ void exp2_pair(uint64_t y2, float& a, float& b) {
     constexpr float kRound = 12582912.0f;
@@ -692,8 +694,8 @@ struct SharedCombine {
 // partials' outputs, whose loads wait for nothing, are on their way.  Bound by
 // latency where rows are few and by the threads' own work where they are many, so
 // with fewer rows there are more threads for them (8, 64, 128 and 256 sequences, 8
-// heads, us a call): kSplit 4 14.2, 58.3, -, 110; kSplit 2 15.4, 55.4, 58.5, 93;
-// one part and four quads a thread 17.7, 62.5, 60, 87.5.
+// heads, us a call): kSplit 4 14.5, 61.2, 66.8, 114; kSplit 2 16.1, 58.1, 60.1, 98.7;
+// one part and four quads a thread 18.2, 65.0, 61.6, 94.4.
 constexpr int kMaxParts = 3 * kAttnMaxCtas;  // two a CTA of the prefix, one a CTA of the own tokens
 template <int kSplit, int kQuads, int kFirst>  // kFirst prefix partials are loaded ahead
 __global__ void __launch_bounds__(256 / kQuads) kv_shared_combine_kernel(const __grid_constant__ SharedCombine p) {
@@ -897,8 +899,8 @@ int hsb_kv_attention_shared(const hsb_kv_pages* prefix, const int32_t* d_prefix_
     // a tile for each warpgroup at least: more CTAs would only leave more partials
     const unsigned units = g.runs * g.tiles, least = g.dual ? (units + 1) / 2 : units;
     const unsigned grid = std::min<unsigned>({least, (unsigned)device_info().sms, kAttnMaxCtas});
-    // idle places pay where a CTA has several times as many tiles (64 x 32768: 63.1 us without, 59.2 with;
-    // 256 x 16461: 94.6 and 92.5)
+    // idle places pay where a CTA has several times as many tiles (64 x 32768: 60.4 us without, 58.4 with;
+    // 256 x 16461: 97.1 and 94.4)
     p.run_cost = units >= 6 * grid ? 2 : 0;
     cudaError_t e = g.dual ? launch_prefix<true>(p, grid, s) : launch_prefix<false>(p, grid, s);
     if (e != cudaSuccess) return record_cuda_error(e, "paged KV attention launch");
