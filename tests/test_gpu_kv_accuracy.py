@@ -189,3 +189,52 @@ def test_attention_channel_by_channel(cuda, fmt, lengths):
             strict(got[b], q[b], kv, TOPS[fmt])
         else:
             assert not got[b].any()
+
+
+@pytest.mark.parametrize("heads,batch,tiles", [(8, 4, 4753), (8, 30, 9000), (8, 1216, 257), (8, 1216, 513)])
+@pytest.mark.parametrize("slope", [0.0, 1.0, -1.0])
+def test_shared_sums_that_end_and_begin_again(cuda, heads, batch, tiles, slope):
+    """Stretches of 257, 486, 257 and 513 tiles: with one M tile the last sum of a single tile leaves one warpgroup
+    none.  Equal weights, or logits that rise or fall by 32 along the prefix (|logit| < 32 + 5)."""
+    rng = np.random.default_rng(47)
+    pages, prefix = 32, tiles * 128 - 5
+    kv = ko.rows(rng, pages * 64, heads, 0.3)
+    kv[:, 0, :, 0] = (np.arange(pages * 64) // 64 * 1.0)[:, None]
+    kv[:, 1] = (1.0 + 0.1 * rng.standard_normal(kv[:, 1].shape)).astype(np.float16)
+    pre, pkv = pool_of(cuda, rng, "f16", heads, pages, kv)
+    total = -(-prefix // 64)
+    table = (np.arange(total) * pages // total).astype(np.int32)
+    counts = counts_of(table, prefix, pages)
+    q = (0.3 * rng.standard_normal((batch, 4 * heads, 128))).astype(np.float16)
+    q[:, :, 0] = slope * np.sqrt(128.0)
+    own, okv = pool_of(cuda, rng, "int8", heads, 1)
+    got = own.attention_shared(dev(q), i32(np.zeros((batch, 1))), i32([2] * batch), pre, i32(table), prefix)
+    own.check()
+    both, pick = np.concatenate([pkv, okv]), sorted({0, 1, batch // 2, batch - 1})
+    counts = np.concatenate([counts, np.arange(64) < 2])
+    want = np.stack([attention(q[b], both, counts) for b in pick])
+    close(got[pick], want, [both], TOL16 + 256 * 8 * 2 * 2.0**-23 + 2 * 15 * 2.0**-23 * 37)
+
+
+@pytest.mark.parametrize("batch", [4, 64, 1216])
+@pytest.mark.parametrize("q0", [1.0, 300.0, -300.0, 60000.0, -60000.0])
+def test_shared_logits_that_grow_far(cuda, batch, q0):
+    """Keys 8 t and one loud query channel: references that pass 2^20 in the middle of a stretch of 16 tiles (or begin
+    above it, or fall).  Neighbouring logits are 0.7 |q0| apart, so all but a few take no weight."""
+    rng = np.random.default_rng(48)
+    heads, prefix = 8, 2048
+    kv = ko.rows(rng, prefix, heads, 0.1)
+    kv[:, 0] = 0
+    kv[:, 0, :, 0] = (8.0 * np.arange(prefix))[:, None]
+    pre, pkv = pool_of(cuda, rng, "f16", heads, prefix // 64, kv)
+    own, _ = pool_of(cuda, rng, "int8", heads, 1)
+    q = np.zeros((batch, 4 * heads, 128), np.float16)
+    q[:, :, 0] = q0
+    q[:, 1::4, 0] = 0.001  # (a row of small logits beside them in each warp)
+    got = own.attention_shared(dev(q), i32(np.zeros((batch, 1))), i32([0] * batch), pre, i32(np.arange(prefix // 64)),
+                               prefix)
+    own.check()
+    pick = sorted({0, batch // 2, batch - 1})
+    want = np.stack([attention(q[b], pkv, np.ones(prefix)) for b in pick])
+    # (|logit| of a row whose neighbours count is below 2^11 |q0| = 1450: 15 roundings of 2^-23 each, twice)
+    close(got[pick], want, [pkv], TOL16 + (2 * 15 * 2.0**-23 * 1450 if q0 == 1.0 else 0.0))
